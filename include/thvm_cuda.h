@@ -323,6 +323,46 @@ int      thvm_cuda_maxpool2x2_index(uint32_t out_val, uint32_t out_idx, uint32_t
  * thvm_argmax (src/ops/_.c:502-524), which reads the whole tensor back first. */
 int      thvm_cuda_argmax_rows(uint32_t out_u32, uint32_t x, uint32_t rows, uint32_t cols);
 
+/* ---- layer operators (no vtable slot) ----
+ * One call each for what a network of fully connected, normalised layers trains and serves with; through the vtable they
+ * are several dispatches with the intermediate tensors in memory.  Operands are contiguous row-major buffers, by id, of one
+ * dtype (THC_F32 or THC_F16); sums are f32 or wider, and f16 results are rounded to nearest even once, when stored.  Work
+ * is queued on the backend's stream and can be recorded into a captured step.  All return 0 = launched, 1 = bad argument
+ * with the reason in thvm_cuda_last_error() and nothing written: an empty shape, a missing, dead or too small buffer, an
+ * unknown dtype or activation, or an output that is also an input or another output (exceptions below).  An id of 0 leaves an
+ * optional operand out. */
+#define THC_ACT_NONE 0
+#define THC_ACT_RELU 1                  /* z > 0 ? z : 0, as the RELU op */
+#define THC_ACT_GELU 2                  /* z (1 + erf(z / sqrt 2)) / 2 */
+#define THC_ACT_SILU 3                  /* z / (1 + e^-z) */
+/* y = act(x w + bias) + residual, for x [M,K], w [K,N], bias [N], residual and y [M,N].  The counterpart of the reference's
+ * linear layer (src/nn/tg_tensor.c:34-88), weights stored (in, out).  `z` (optional output, [M,N]) keeps x w + bias for the
+ * backward pass; bias and residual are optional; y may be the residual's buffer. */
+int      thvm_cuda_linear(uint32_t y, uint32_t z, uint32_t x, uint32_t w, uint32_t bias, uint32_t residual,
+                          uint32_t M, uint32_t K, uint32_t N, uint32_t act, uint32_t dtype);
+/* Gradients of the above: with dz = dy act'(z), dx = dz w^T [M,K], dw = x^T dz [K,N], dbias = sum of dz over rows [N].  Each
+ * output is optional (one at least); x is needed for dw, w for dx, z unless act is THC_ACT_NONE (for THC_ACT_RELU a y that
+ * had no residual serves as z).  The residual's gradient is dy itself. */
+int      thvm_cuda_linear_backward(uint32_t dx, uint32_t dw, uint32_t dbias, uint32_t dy, uint32_t z, uint32_t x, uint32_t w,
+                                   uint32_t M, uint32_t K, uint32_t N, uint32_t act, uint32_t dtype);
+/* Layer norm over the last dim: y = (x - mean) rstd gamma + beta with rstd = 1 / sqrt(var + eps), var the mean squared
+ * deviation.  gamma and beta [cols] are optional; mean and rstd (optional outputs, f32 [rows] for either dtype) are what the
+ * backward pass takes.  y may be x's buffer. */
+int      thvm_cuda_layernorm(uint32_t y, uint32_t mean, uint32_t rstd, uint32_t x, uint32_t gamma, uint32_t beta,
+                             uint32_t rows, uint32_t cols, float eps, uint32_t dtype);
+/* Gradients of the above: dx [rows,cols], dgamma and dbeta [cols] (each optional, one at least).  gamma optional; dx may be
+ * dy's or x's buffer.  Column sums are added in a fixed order: the same call gives the same bits. */
+int      thvm_cuda_layernorm_backward(uint32_t dx, uint32_t dgamma, uint32_t dbeta, uint32_t dy, uint32_t x, uint32_t gamma,
+                                      uint32_t mean, uint32_t rstd, uint32_t rows, uint32_t cols, uint32_t dtype);
+/* Orthogonalises an f32 matrix by Newton-Schulz products: X = x / (|x|_F + 1e-7), then `steps` (1..32) times
+ * X = a X + (b S + c S S) X with S = X X^T (for rows > cols: X = a X + X (b S + c S S), S = X^T X) and
+ * a, b, c = 3.4445, -4.7750, 2.0315.  Dimensions up to 2^20; `out` may be x's buffer. */
+int      thvm_cuda_newton_schulz(uint32_t out, uint32_t x, uint32_t rows, uint32_t cols, uint32_t steps);
+/* In-place optimizer step of an f32 weight matrix, beside adam_step: mom = mu mom + grad; u = nesterov ? grad + mu mom : mom;
+ * param = param (1 - lr weight_decay) - lr sqrt(max(1, rows / cols)) newton_schulz(u).  rows = in, cols = out. */
+int      thvm_cuda_muon_step(uint32_t param, uint32_t grad, uint32_t momentum, uint32_t rows, uint32_t cols,
+                             float lr, float mu, float weight_decay, uint32_t nesterov, uint32_t steps);
+
 /* ---- allocation-free variant (no counterpart in the reference) ----
  * out[c] = sum over b and i of x[b][c][i] for a contiguous f32 tensor x[B][C][HW]
  * (the batch-norm channel statistic), computed by the same split reduce kernels

@@ -93,6 +93,12 @@ SYMBOLS = {
     "thvm_cuda_graph_input_bytes": (_u64, [C.c_int, C.c_int]),
     "thvm_cuda_maxpool2x2_index": (C.c_int, [_u32, _u32, _u32, _u32, _u32, _u32]),
     "thvm_cuda_argmax_rows": (C.c_int, [_u32, _u32, _u32, _u32]),
+    "thvm_cuda_linear": (C.c_int, [_u32] * 11),
+    "thvm_cuda_linear_backward": (C.c_int, [_u32] * 12),
+    "thvm_cuda_layernorm": (C.c_int, [_u32] * 8 + [C.c_float, _u32]),
+    "thvm_cuda_layernorm_backward": (C.c_int, [_u32] * 11),
+    "thvm_cuda_newton_schulz": (C.c_int, [_u32] * 5),
+    "thvm_cuda_muon_step": (C.c_int, [_u32] * 5 + [C.c_float] * 3 + [_u32] * 2),
     "thvm_cuda_channel_sums_noalloc": (C.c_int, [_vp, _vp, _u32, _u32, _u32, _vp]),
     "thvm_cuda_signature": (_u64, [C.POINTER(abi.FusedOp), _u32, C.POINTER(_PV), _vp, _u32,
                                    C.POINTER(abi.Shape), C.POINTER(abi.ReduceSpec)]),

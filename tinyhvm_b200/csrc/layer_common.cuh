@@ -1,0 +1,72 @@
+// layer_common.cuh — what the layer operators (layernorm.cu, linear.cu, muon.cu) share: loads and stores of one to eight
+// neighbouring values as f32, block sums, and the activations with their slopes.
+//
+// f16 values are rounded to nearest even when they are stored.  (The dispatch path rounds half up on the dropped bits,
+// because it is compared bit for bit with the reference; these operators have no counterpart there.)
+#pragma once
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+#include "../../include/thvm_cuda.h"
+
+namespace thc {
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ void put_f32(float *p, float v) { *p = v; }
+__device__ __forceinline__ void put_f32(__half *p, float v) { *p = __float2half_rn(v); }
+
+// 16 bytes hold this many values
+template <typename T> struct Vec16 { static constexpr int n = 16 / (int)sizeof(T); };
+
+// V neighbouring values; V is 1 or Vec16<T>::n (p then 16-byte aligned)
+template <int V> __device__ __forceinline__ void load_vec(const float *p, float (&v)[V]) {
+    if constexpr (V == 4) { const float4 q = *reinterpret_cast<const float4 *>(p); v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w; }
+    else { v[0] = *p; }
+}
+template <int V> __device__ __forceinline__ void load_vec(const __half *p, float (&v)[V]) {
+    if constexpr (V == 8) {
+        const uint4 q = *reinterpret_cast<const uint4 *>(p);
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) { const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i])); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
+    } else { v[0] = __half2float(*p); }
+}
+template <int V> __device__ __forceinline__ void store_vec(float *p, const float (&v)[V]) {
+    if constexpr (V == 4) *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    else *p = v[0];
+}
+template <int V> __device__ __forceinline__ void store_vec(__half *p, const float (&v)[V]) {
+    if constexpr (V == 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) { const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]); w[i] = *reinterpret_cast<const uint32_t *>(&h); }
+        *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else { *p = __float2half_rn(v[0]); }
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// ---- activations (thvm_cuda_linear): value and slope at z ----
+__device__ __forceinline__ float act_value(uint32_t act, float z) {
+    switch (act) {
+        case THC_ACT_RELU: return z > 0.0f ? z : 0.0f;                       // as the RELU op of the dispatch path: NaN gives 0
+        case THC_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+        case THC_ACT_SILU: return z / (1.0f + expf(-z));                     // z = -inf: -inf / inf is NaN, as the formula says
+        default:           return z;
+    }
+}
+__device__ __forceinline__ float act_slope(uint32_t act, float z) {
+    switch (act) {
+        case THC_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
+        case THC_ACT_GELU: return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+        case THC_ACT_SILU: { const float s = 1.0f / (1.0f + expf(-z)); return s * (1.0f + z * (1.0f - s)); }
+        default:           return 1.0f;
+    }
+}
+
+}  // namespace thc
