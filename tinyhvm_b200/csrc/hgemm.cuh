@@ -1,0 +1,432 @@
+// hgemm.cuh — products of f16 planes on the tensor cores, for the layer operators (included by linear.cu and muon.cu).
+//
+//   acc(m, n) = sum over k of A(m,k) B(n,k),   A = A_hi + A_lo,  B = B_hi + B_lo      (low planes optional)
+//
+// An f32 operand travels as two f16 planes of x 2^s: hi = f16(x 2^s) and lo = f16(x 2^s - hi).  f16 holds 11 bits, the
+// remainder is at most half a step and has a sign, so hi + lo is x to 2^-24 relative, f32's own half step, as long as
+// the scaled value is not so small that lo falls below f16's smallest step, 2^-24: the scale puts the largest value of a row in
+// [2^14, 2^15), which leaves 2^-40 of that as the floor.  A B is then A_hi B_lo + A_lo B_hi + A_hi B_hi (the fourth
+// product is below 2^-24): three f16 MMAs, where three tf32 MMAs would run at half their rate and keep 2^-21.
+//
+// The tensor core truncates when it adds to an accumulator, so a long sum drifts towards zero by about 2^-24 per add.
+// Here an accumulator lives for `chunk` blocks of 64 k only (2 with low planes, 8 without): eight epilogue warps then take it from
+// tensor memory and add it, rounded, to f32 sums in registers, while the MMAs of the next chunk fill the other of
+// two accumulators.  Within a block of k the small products go first.
+//
+// A CTA pair (cta_group::2) computes a 256 x NT tile, NT = 256 or 128: each CTA holds 128 rows of A, half of B's
+// columns, and the accumulators of its own rows.  Roles: warps 0-7 epilogue, warp 8 tile loads, warp 9 (first CTA) MMAs.  The pairs are
+// persistent and walk over the tiles, so the next tile's loads and MMAs run under this one's epilogue.
+//
+// Operands may lie either way round, as the matrix descriptors allow for f16: k along memory rows (boxes of 64 k x rows),
+// or m / n along memory rows (boxes of 64 rows x 64 k), so nothing is ever transposed.
+//
+// Every wait is bounded.  A wait that runs out raises status bit 8 and ends the kernel after its copies in flight.
+#pragma once
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <string.h>
+#include <unordered_map>
+#include "layer_common.cuh"
+#include "state.h"
+
+namespace thc {
+namespace hg {
+
+constexpr uint32_t EPI_WARPS = 8, TMA_WARP = 8, MMA_WARP = 9, THREADS = 320;
+constexpr uint32_t KB = 64;                                // k of a block: 128 bytes, the swizzle's width
+constexpr uint32_t A_PLANE = 128 * 128;                    // bytes of one CTA's A plane of a block
+constexpr uint32_t RING_BYTES = 196608, STAGING = EPI_WARPS * 4096;
+constexpr uint32_t MAX_STAGES = 8;
+constexpr uint32_t WAIT_LIMIT = 1u << 24;
+constexpr int STATUS_TIMEOUT = 8;
+
+struct Shared {
+    unsigned long long full[MAX_STAGES], empty[MAX_STAGES], acc_full[2], acc_empty[2];
+    uint32_t tmem;
+    int abort_flag;
+};
+constexpr size_t SMEM = 1024 + RING_BYTES + STAGING + sizeof(Shared);
+
+struct Shape {
+    uint32_t M, N, K;
+    uint32_t row_tiles, col_tiles, tiles;                  // tiles: of all splits, below the diagonal left out when `upper`
+    uint32_t blocks, split_blocks, chunk;                  // blocks of 64 k: in all, per split, per chunk
+    uint32_t splits;
+    uint32_t stages, stage_bytes, a_bytes;
+    uint32_t a_mn, b_mn, a_lo, b_lo, upper;
+    int *status;
+};
+struct Maps { CUtensorMap a[2], b[2]; };
+
+// ---- PTX ----
+__device__ __forceinline__ uint32_t smem32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) { uint32_t r; asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank)); return r; }
+__device__ __forceinline__ uint32_t cluster_cta() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(n) : "memory"); }
+__device__ __forceinline__ void bar_arrive(uint32_t cluster_addr) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory"); }
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
+// false after WAIT_LIMIT polls or when another thread of this CTA gave up
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
+    for (uint32_t it = 0; it < WAIT_LIMIT; ++it) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
+        if ((it & 255u) == 255u && *abort_flag) return false;
+    }
+    *abort_flag = 1;
+    return false;
+}
+// box at (x, y) of the map into this CTA's shared memory, signalled on a barrier of the pair's first CTA
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, uint32_t bar, uint32_t x, uint32_t y) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"((int)x), "r"((int)y) : "memory");
+}
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void commit_both(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+// 128-byte-swizzled operand.  k along rows: 8-row groups 1024 bytes apart.  m / n along rows: 64-value blocks 8192 bytes apart, groups of
+// 8 k 1024 bytes apart.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, uint32_t mn) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(mn ? 8192u >> 4 : 1u) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void acc_load(uint32_t addr, uint32_t (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(addr) : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+struct Tile { uint32_t m0, n0, z, blocks, block0; };
+// Tiles in order: split, then bands of 8 row tiles, columns, rows of the band: the tiles in flight share few operand panels.
+template <uint32_t NT> __device__ __forceinline__ Tile tile_of(const Shape &S, uint32_t t) {
+    Tile r;
+    uint32_t row, col;
+    if (S.upper) {                                         // row by row from the diagonal on
+        row = 0; col = t;
+        for (;;) {
+            const uint32_t first = row * 256u / NT, n = S.col_tiles - first;
+            if (col < n) { col += first; break; }
+            col -= n; row++;
+        }
+        r.z = 0;
+    } else {
+        const uint32_t per = S.row_tiles * S.col_tiles;
+        r.z = t / per;
+        const uint32_t u = t - r.z * per, band = u / (8u * S.col_tiles), v = u - band * 8u * S.col_tiles;
+        const uint32_t h = S.row_tiles - band * 8u < 8u ? S.row_tiles - band * 8u : 8u;
+        col = v / h; row = band * 8u + (v - col * h);
+    }
+    r.m0 = row * 256u; r.n0 = col * NT;
+    r.block0 = r.z * S.split_blocks;
+    r.blocks = S.blocks - r.block0 < S.split_blocks ? S.blocks - r.block0 : S.split_blocks;
+    return r;
+}
+
+// Epi: what happens to a finished sum.  put(m, n, v, z) is called with n running along the lanes; with Epi::mirror,
+// mirror(n, m, v) too, m running along the lanes, for the transposed place of a symmetric product.
+template <uint32_t NT, class Epi>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+k_hgemm(const __grid_constant__ Shape S, const __grid_constant__ Maps maps, const __grid_constant__ Epi epi) {
+    extern __shared__ uint8_t raw[];
+    uint8_t *base = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    Shared &sh = *reinterpret_cast<Shared *>(base + RING_BYTES + STAGING);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, rank = cluster_cta();
+    const uint32_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    volatile int *abort_flag = &sh.abort_flag;
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < MAX_STAGES; s++) { bar_init(smem32(&sh.full[s]), 1); bar_init(smem32(&sh.empty[s]), 1); }
+        for (int b = 0; b < 2; b++) { bar_init(smem32(&sh.acc_full[b]), 1); bar_init(smem32(&sh.acc_empty[b]), 2 * EPI_WARPS); }
+        sh.abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == MMA_WARP) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem32(&sh.tmem)), "r"(2u * NT) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = sh.tmem;
+    const uint32_t ring = smem32(base);
+    constexpr uint32_t B_PLANE = NT / 2 * 128;             // bytes of this CTA's B plane of a block
+
+    if (warp < EPI_WARPS) {
+        // ================= epilogue: rows of this CTA, quadrant warp % 4; columns half warp / 4 =================
+        constexpr uint32_t COLS = NT / 2;
+        const uint32_t q = warp & 3u, half = warp >> 2;
+        float *st = reinterpret_cast<float *>(base + RING_BYTES) + warp * 1024u;
+        Epi e = epi;                                       // (keeps what belongs to the lane's column)
+        bool ok = true;
+        uint32_t c = 0;                                    // chunks so far
+        for (uint32_t t = pair; t < S.tiles && ok; t += pairs) {
+            const Tile T = tile_of<NT>(S, t);
+            float acc[COLS];
+#pragma unroll
+            for (uint32_t i = 0; i < COLS; i++) acc[i] = 0.0f;
+            for (uint32_t kb = 0; kb < T.blocks && ok; kb += S.chunk, c++) {
+                const uint32_t buf = c & 1u;
+                ok = bar_wait(smem32(&sh.acc_full[buf]), (c >> 1) & 1u, abort_flag);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                for (uint32_t j = 0; j < COLS / 32; j++) {
+                    uint32_t r[32];
+                    acc_load(tmem + ((q * 32u) << 16) + buf * NT + half * COLS + j * 32u, r);
+#pragma unroll
+                    for (uint32_t i = 0; i < 32; i++) acc[j * 32 + i] += __uint_as_float(r[i]);
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) bar_arrive(in_cta(smem32(&sh.acc_empty[buf]), 0));
+            }
+            if (!ok) break;
+            const uint32_t m0 = T.m0 + rank * 128u + q * 32u, n0 = T.n0 + half * COLS;
+#pragma unroll
+            for (uint32_t j = 0; j < COLS / 32; j++) {
+                const uint32_t n1 = n0 + j * 32u;
+                if (n1 >= S.N || m0 >= S.M) continue;
+                if constexpr (Epi::mirrors) {
+                    if (S.upper) {
+#pragma unroll
+                        for (uint32_t i = 0; i < 32; i++)  // this thread's row m0 + lane: neighbours in the transposed row
+                            if (m0 + lane < n1 + i && n1 + i < S.N) e.mirror(n1 + i, m0 + lane, acc[j * 32 + i]);
+                    }
+                }
+                __syncwarp();
+#pragma unroll
+                for (uint32_t i = 0; i < 32; i++) st[lane * 32u + (i ^ lane)] = acc[j * 32 + i];
+                __syncwarp();
+                const uint32_t n = n1 + lane;
+                const uint32_t rows = S.M - m0 < 32u ? S.M - m0 : 32u;
+                if (n < S.N) {
+                    e.column(n);
+#pragma unroll 4
+                    for (uint32_t r = 0; r < rows; r++) {
+                        const float v = st[r * 32u + (lane ^ r)];
+                        if (!(Epi::mirrors && S.upper && m0 + r > n)) e.put(m0 + r, n, v, T.z);
+                    }
+                }
+            }
+        }
+    } else if (warp == TMA_WARP) {
+        // ================= tile loads: one thread per CTA =================
+        if (lane == 0) {
+            bool ok = true;
+            uint32_t it = 0, s = 0, use = 0;
+            const uint32_t planes_a = 1u + S.a_lo, planes_b = 1u + S.b_lo;
+            for (uint32_t t = pair; t < S.tiles && ok; t += pairs) {
+                const Tile T = tile_of<NT>(S, t);
+                const uint32_t m = T.m0 + rank * 128u, n = T.n0 + rank * (NT / 2);
+                for (uint32_t kb = 0; kb < T.blocks; kb++) {
+                    if (use) ok = bar_wait(smem32(&sh.empty[s]), (use - 1) & 1u, abort_flag);
+                    if (!ok) break;
+                    const uint32_t bar = in_cta(smem32(&sh.full[s]), 0), k = (T.block0 + kb) * KB;
+                    if (rank == 0) bar_expect(smem32(&sh.full[s]), 2u * S.stage_bytes);
+                    uint32_t dst = ring + s * S.stage_bytes;
+                    for (uint32_t p = 0; p < planes_a; p++, dst += A_PLANE) {
+                        if (S.a_mn) { load_box(dst, &maps.a[p], bar, m, k); load_box(dst + 8192u, &maps.a[p], bar, m + 64u, k); }
+                        else load_box(dst, &maps.a[p], bar, k, m);
+                    }
+                    for (uint32_t p = 0; p < planes_b; p++, dst += B_PLANE) {
+                        if (S.b_mn) {
+#pragma unroll
+                            for (uint32_t j = 0; j < NT / 128; j++) load_box(dst + j * 8192u, &maps.b[p], bar, n + j * 64u, k);
+                        } else load_box(dst, &maps.b[p], bar, k, n);
+                    }
+                    it++;
+                    if (++s == S.stages) { s = 0; use++; }
+                }
+            }
+            if (!ok && rank == 0) {
+                // give the copies in flight (both CTAs' signal here) time to land before shared memory is given up
+                int never = 0;
+                const uint32_t n = it < S.stages ? it : S.stages;
+                for (uint32_t i = it - n; i < it; i++) bar_wait(smem32(&sh.full[i % S.stages]), (i / S.stages) & 1u, &never);
+            }
+        }
+        __syncwarp();
+    } else if (rank == 0) {
+        // ================= MMAs: one thread, for the pair =================
+        if (lane == 0) {
+            const uint32_t idesc = (1u << 4) | (S.a_mn << 15) | (S.b_mn << 16) | ((NT >> 3) << 17) | ((256u >> 4) << 24);   // f32 sums of f16 products
+            const uint64_t step_a = S.a_mn ? 2048u >> 4 : 32u >> 4, step_b = S.b_mn ? 2048u >> 4 : 32u >> 4;                 // 16 k further
+            bool ok = true;
+            uint32_t s = 0, use = 0, c = 0;
+            for (uint32_t t = pair; t < S.tiles && ok; t += pairs) {
+                const Tile T = tile_of<NT>(S, t);
+                for (uint32_t kb = 0; kb < T.blocks && ok; kb += S.chunk, c++) {
+                    const uint32_t buf = c & 1u, d = tmem + buf * NT;
+                    if (c >= 2) ok = bar_wait(smem32(&sh.acc_empty[buf]), ((c >> 1) - 1) & 1u, abort_flag);
+                    const uint32_t end = T.blocks - kb < S.chunk ? T.blocks - kb : S.chunk;
+                    uint32_t more = 0;
+                    for (uint32_t i = 0; i < end && ok; i++) {
+                        ok = bar_wait(smem32(&sh.full[s]), use & 1u, abort_flag);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint32_t sa = ring + s * S.stage_bytes, sb = sa + S.a_bytes;
+                        const uint64_t a_hi = operand_desc(sa, S.a_mn), b_hi = operand_desc(sb, S.b_mn);
+                        if (S.a_lo) {
+                            const uint64_t a_lo = operand_desc(sa + A_PLANE, S.a_mn);
+#pragma unroll
+                            for (uint32_t k = 0; k < 4; k++) { mma(d, a_lo + k * step_a, b_hi + k * step_b, idesc, more); more = 1; }
+                        }
+                        if (S.b_lo) {
+                            const uint64_t b_lo = operand_desc(sb + B_PLANE, S.b_mn);
+#pragma unroll
+                            for (uint32_t k = 0; k < 4; k++) { mma(d, a_hi + k * step_a, b_lo + k * step_b, idesc, more); more = 1; }
+                        }
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; k++) { mma(d, a_hi + k * step_a, b_hi + k * step_b, idesc, more); more = 1; }
+                        commit_both(smem32(&sh.empty[s]));
+                        if (++s == S.stages) { s = 0; use++; }
+                    }
+                    if (ok) commit_both(smem32(&sh.acc_full[buf]));
+                }
+            }
+        }
+        __syncwarp();
+    }
+
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync();
+    if (threadIdx.x == 0 && sh.abort_flag) atomicOr(S.status, STATUS_TIMEOUT);
+    if (warp == MMA_WARP) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2u * NT) : "memory");
+    }
+}
+
+// Sums of a split product: partial[z][m][n] in split order, then the epilogue.
+struct PartialEpi {
+    static constexpr bool mirrors = false;
+    float *partial; uint64_t mn; uint32_t N;
+    __device__ void column(uint32_t) const {}
+    __device__ void mirror(uint32_t, uint32_t, float) const {}
+    __device__ void put(uint32_t m, uint32_t n, float v, uint32_t z) const { partial[z * mn + (uint64_t)m * N + n] = v; }
+};
+template <class Epi>
+__global__ void __launch_bounds__(256)
+k_hgemm_fold(const float *partial, uint32_t splits, uint32_t M, uint32_t N, const __grid_constant__ Epi epi) {
+    const uint32_t n = blockIdx.x * 128 + (threadIdx.x & 127u);
+    if (n >= N) return;
+    Epi e = epi;
+    e.column(n);
+    for (uint32_t m = blockIdx.y * 2 + (threadIdx.x >> 7); m < M; m += gridDim.y * 2) {
+        float v = 0.0f;
+        for (uint32_t z = 0; z < splits; z++) v += partial[((uint64_t)z * M + m) * N + n];
+        e.put(m, n, v, 0);
+    }
+}
+
+// ---- host ----
+// One operand: `rows` x `cols` f16 planes in memory, rows `pitch` values apart (a multiple of 8, base 16-byte aligned).  mn: the rows run
+// along k; otherwise along the operand's m or n.
+struct Operand { const __half *hi, *lo; uint64_t pitch; bool mn; };
+
+typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
+                                CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static void make_map(CUtensorMap *m, const __half *base, uint64_t inner, uint64_t outer, uint64_t pitch, uint32_t box_outer) {
+    static EncodeTiled fn = nullptr;
+    if (!fn) {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        THC_CUDA_OK(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q));
+        if (q != cudaDriverEntryPointSuccess) fatal("cuTensorMapEncodeTiled is not in this driver");
+        fn = (EncodeTiled)p;
+    }
+    const cuuint64_t dims[2] = {inner, outer}, strides[1] = {pitch * 2};
+    const cuuint32_t box[2] = {64, box_outer}, one[2] = {1, 1};
+    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<__half *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) fatal("tensor map of %llu x %llu values, pitch %llu: error %d", (unsigned long long)outer, (unsigned long long)inner, (unsigned long long)pitch, (int)r);
+}
+static void operand_maps(CUtensorMap (&maps)[2], const Operand &o, uint32_t rows, uint32_t K, uint32_t box_rows) {
+    for (int p = 0; p < 2; p++) {
+        const __half *base = p && o.lo ? o.lo : o.hi;
+        if (o.mn) make_map(&maps[p], base, rows, K, o.pitch, KB);
+        else make_map(&maps[p], base, K, rows, o.pitch, box_rows);
+    }
+}
+
+struct Plan { uint32_t nt, splits; uint64_t partial_bytes; };
+// Tile width and splits for an M x N product over K.  Wide tiles halve the traffic of A's panels, but a grid that leaves
+// pairs idle loses more: narrow ones then, and below half a grid K is split as well, into runs of at least 4 blocks of 64.
+static Plan plan(uint32_t M, uint32_t N, uint32_t K, bool may_split) {
+    const uint32_t pairs = (uint32_t)g.sm_count / 2, rows = (M + 255) / 256;
+    Plan p;
+    p.nt = (uint64_t)rows * ((N + 255) / 256) >= pairs ? 256 : 128;
+    const uint64_t tiles = (uint64_t)rows * ((N + p.nt - 1) / p.nt);
+    const uint32_t blocks = (K + KB - 1) / KB;
+    uint64_t s = may_split ? pairs / tiles : 1;
+    if (s > blocks / 4) s = blocks / 4;
+    if (s < 1) s = 1;
+    const uint32_t per = (uint32_t)((blocks + s - 1) / s);
+    p.splits = (blocks + per - 1) / per;
+    p.partial_bytes = p.splits > 1 ? (uint64_t)p.splits * M * N * 4 : 0;
+    return p;
+}
+
+template <uint32_t NT, class Epi>
+static void launch(const Shape &S, const Maps &maps, const Epi &epi, const char *name) {
+    static bool ready = false;
+    if (!ready) { THC_CUDA_OK(cudaFuncSetAttribute(k_hgemm<NT, Epi>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM)); ready = true; }
+    const uint32_t pairs = (uint32_t)g.sm_count / 2;
+    profile_begin();
+    k_hgemm<NT, Epi><<<2 * (S.tiles < pairs ? S.tiles : pairs), THREADS, SMEM, g.stream>>>(S, maps, epi);
+    after_launch(name);
+}
+
+// A (M rows) times B (N rows) over K.  `partial`: plan.partial_bytes of scratch.  `upper`: a symmetric product (A = B): tiles
+// below the diagonal are left out and the epilogue mirrors the others.
+template <class Epi>
+static void product(const Operand &A, const Operand &B, uint32_t M, uint32_t N, uint32_t K, const Plan &p, float *partial, const Epi &epi, bool upper, const char *name) {
+    Shape S;
+    memset(&S, 0, sizeof S);
+    S.M = M; S.N = N; S.K = K;
+    S.row_tiles = (M + 255) / 256; S.col_tiles = (N + p.nt - 1) / p.nt;
+    S.blocks = (K + KB - 1) / KB;
+    S.split_blocks = (S.blocks + p.splits - 1) / p.splits;
+    S.splits = p.splits;
+    S.a_mn = A.mn; S.b_mn = B.mn; S.a_lo = A.lo != nullptr; S.b_lo = B.lo != nullptr;
+    S.chunk = S.a_lo || S.b_lo ? 2 : 8;
+    S.a_bytes = A_PLANE * (1 + S.a_lo);
+    S.stage_bytes = S.a_bytes + p.nt / 2 * 128 * (1 + S.b_lo);
+    S.stages = RING_BYTES / S.stage_bytes;
+    if (S.stages > MAX_STAGES) S.stages = MAX_STAGES;
+    S.upper = upper;
+    S.tiles = S.row_tiles * S.col_tiles * p.splits;
+    if (upper) { S.tiles = 0; for (uint32_t r = 0; r < S.row_tiles; r++) S.tiles += S.col_tiles - r * 256 / p.nt; }
+    S.status = g.dev_status;
+    Maps maps;
+    operand_maps(maps.a, A, M, K, 128);
+    operand_maps(maps.b, B, N, K, p.nt / 2);
+    if (p.splits > 1) {
+        const PartialEpi pe{partial, (uint64_t)M * N, N};
+        if (p.nt == 256) launch<256>(S, maps, pe, name); else launch<128>(S, maps, pe, name);
+        profile_begin();
+        k_hgemm_fold<Epi><<<dim3((N + 127) / 128, (M + 7) / 8 < 4096 ? (M + 7) / 8 : 4096), 256, 0, g.stream>>>(partial, p.splits, M, N, epi);
+        after_launch("layer_fold");
+    } else if (p.nt == 256) launch<256>(S, maps, epi, name);
+    else launch<128>(S, maps, epi, name);
+}
+
+}  // namespace hg
+}  // namespace thc

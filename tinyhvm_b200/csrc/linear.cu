@@ -2,6 +2,7 @@
 //
 //   forward   z = x w + bias,  y = act(z) + residual                    x [M,K], w [K,N] (in, out: as the framework stores weights)
 //   backward  dz = dy act'(z);  dx = dz w^T;  dw = x^T dz;  dbias = sum over rows of dz
+#include "hgemm.cuh"
 #include "layer_common.cuh"
 #include "layer_host.h"
 #include "state.h"
@@ -31,100 +32,376 @@ bool layer_buffers(const char *who, const uint32_t *ins, const uint64_t *in_need
     return true;
 }
 
-// ---- contraction on the CUDA cores: C(m,n) = sum_k A(m,k) B(k,n) through element strides ----
-struct Strided { const void *p; uint64_t sm, sk; };    // sm: along m (or n), sk: along k
-template <typename TA, typename TB, class Epi>
-__global__ void __launch_bounds__(256)
-k_product(Strided A, Strided B, Epi epi, uint32_t M, uint32_t N, uint32_t K) {
-    __shared__ float As[16][65], Bs[16][65];
-    const uint32_t m0 = blockIdx.y * 64, n0 = blockIdx.x * 64, tx = threadIdx.x & 15u, ty = threadIdx.x >> 4;
-    float acc[4][4] = {};
-    for (uint32_t k0 = 0; k0 < K; k0 += 16) {
-        for (uint32_t u = threadIdx.x; u < 1024; u += 256) {
-            // neighbouring threads walk along whichever index is dense
-            const uint32_t ma = A.sk == 1 ? u >> 4 : u & 63u, ka = A.sk == 1 ? u & 15u : u >> 6;
-            const uint32_t nb = B.sk == 1 ? u >> 4 : u & 63u, kb = B.sk == 1 ? u & 15u : u >> 6;
-            As[ka][ma] = m0 + ma < M && k0 + ka < K ? to_f32(((const TA *)A.p)[(m0 + ma) * A.sm + (k0 + ka) * A.sk]) : 0.0f;
-            Bs[kb][nb] = n0 + nb < N && k0 + kb < K ? to_f32(((const TB *)B.p)[(n0 + nb) * B.sm + (k0 + kb) * B.sk]) : 0.0f;
-        }
-        __syncthreads();
+// ---- operands ----
+// f32 operands become planes of x 2^s (hgemm.cuh).  The scale belongs to a row of memory, so that a row is read once, kept in
+// registers while its largest value is found, and written as planes.  Where the contraction runs along those rows
+// (x, dz and, for dx, w) the result is scaled back in the epilogue; where it runs across them, the other operand takes the
+// inverse scales before it is split itself:
+//   forward   w [K,N] by rows k: w' = w 2^s_k;           x' = x 2^-s_k, then scaled by its own rows m
+//   dw        dz [M,N] by rows m: dz' = dz 2^s_m;        x' = x 2^-s_m, then scaled by its columns k (over m)
+// Values below 2^-40 of the largest in their row (column) are rounded to that step.  An infinity in an f32 operand of the
+// matrix engine gives NaN where it takes part, as in the framework's other contractions: its low part is no number.
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }       // -126 <= e <= 127
+__device__ __forceinline__ float finite_abs(float v) { v = fabsf(v); return v <= 3.402823466e38f ? v : 0.0f; }
+// the exponent s that puts `top` into [2^14, 2^15); rows below 2^-112 keep fewer bits
+__device__ __forceinline__ int scale_for(float top) {
+    if (top == 0.0f) return 0;
+    const int s = 14 - ((int)(__float_as_uint(top) >> 23) - 127);
+    return s > 126 ? 126 : s;
+}
+template <int VEC> __device__ __forceinline__ void store_half(__half *p, const float (&v)[VEC]) {
+    if constexpr (VEC == 4) {
+        const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+        *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+    } else *p = __float2half_rn(v[0]);
+}
+template <int VEC> __device__ __forceinline__ void load4(const float *p, float (&v)[VEC]) {
+    if constexpr (VEC == 4) { const float4 q = *reinterpret_cast<const float4 *>(p); v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w; }
+    else v[0] = *p;
+}
+template <int VEC> __device__ __forceinline__ void load4(const __half *p, float (&v)[VEC]) {
+    if constexpr (VEC == 4) {
+        const uint2 q = *reinterpret_cast<const uint2 *>(p);
+        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&q.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&q.y));
+        v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+    } else v[0] = __half2float(*p);
+}
+// hi and lo of v 2^s
+template <int VEC> __device__ __forceinline__ void put_planes(__half *hi, __half *lo, const float (&v)[VEC], float scale) {
+    float h[VEC], l[VEC];
 #pragma unroll
-        for (int k = 0; k < 16; k++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] += As[k][ty * 4 + i] * Bs[k][tx + 16 * j];
-        __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const uint32_t m = m0 + ty * 4 + i, n = n0 + tx + 16 * j;
-            if (m < M && n < N) epi(m, n, acc[i][j]);
-        }
+    for (int j = 0; j < VEC; j++) { const float x = v[j] * scale; h[j] = __half2float(__float2half_rn(x)); l[j] = x - h[j]; }
+    store_half<VEC>(hi, h);
+    if (lo) store_half<VEC>(lo, l);
 }
 
-template <typename T> struct LinearEpi {
-    T *y, *z; const T *bias, *residual; uint32_t act, N;
-    __device__ void operator()(uint32_t m, uint32_t n, float v) const {
-        const uint64_t at = (uint64_t)m * N + n;
-        if (bias) v += to_f32(bias[n]);
-        if (z) put_f32(z + at, v);
-        v = act_value(act, v);
-        if (residual) v += to_f32(residual[at]);
-        put_f32(y + at, v);
+// what a row's values are
+template <typename T> struct RowsOf {                  // a matrix, its columns times 2^-shift
+    const T *p; const int *shift; uint32_t cols;
+    template <int VEC> __device__ void load(uint64_t row, uint32_t c, float (&v)[VEC]) const {
+        load4<VEC>(p + row * cols + c, v);
+        if (shift) {
+#pragma unroll
+            for (int j = 0; j < VEC; j++) v[j] *= pow2(-shift[c + j]);
+        }
     }
 };
-template <typename T> struct PlainEpi {
-    T *c; uint32_t N;
-    __device__ void operator()(uint32_t m, uint32_t n, float v) const { put_f32(c + (uint64_t)m * N + n, v); }
+template <typename T> struct GradOf {                  // dz = dy act'(z)
+    const T *dy, *z; uint32_t cols, act;
+    template <int VEC> __device__ void load(uint64_t row, uint32_t c, float (&v)[VEC]) const {
+        load4<VEC>(dy + row * cols + c, v);
+        if (act != THC_ACT_NONE) {
+            float q[VEC];
+            load4<VEC>(z + row * cols + c, q);
+#pragma unroll
+            for (int j = 0; j < VEC; j++) v[j] *= act_slope(act, q[j]);
+        }
+    }
 };
 
-template <typename TA, typename TB, class Epi>
-static void product(Strided A, Strided B, Epi epi, uint32_t M, uint32_t N, uint32_t K) {
-    k_product<TA, TB, Epi><<<dim3((N + 63) / 64, (M + 63) / 64), 256, 0, g.stream>>>(A, B, epi, M, N, K);
-}
+struct Planes { __half *hi, *lo; uint64_t pitch; int *exps; float *sums; };   // any of hi, lo, exps, sums may be null; exps null: unscaled
 
-// dz = dy act'(z) in f32
-template <typename T>
-__global__ void __launch_bounds__(256)
-k_dz(float *dz, const T *dy, const T *z, uint32_t act, uint64_t n) {
-    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += gridDim.x * 256ull) dz[i] = to_f32(dy[i]) * (z ? act_slope(act, to_f32(z[i])) : 1.0f);
+__device__ __forceinline__ float block_max(float v, float *red) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = red[0];
+#pragma unroll
+    for (int w = 1; w < 8; w++) v = fmaxf(v, red[w]);
+    return v;
 }
+// Blocks walk over rows, U units of VEC values a thread in registers; sums[block][cols] = the block's column sums.
+template <class Src, int VEC, int U>
+__global__ void __launch_bounds__(256)
+k_split_rows(const Src src, const Planes out, uint32_t rows, uint32_t cols) {
+    __shared__ float red[8];
+    float sum[U][VEC];
+#pragma unroll
+    for (int i = 0; i < U; i++)
+#pragma unroll
+        for (int j = 0; j < VEC; j++) sum[i][j] = 0.0f;
+    for (uint64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        float v[U][VEC];
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            const uint32_t c = (threadIdx.x + 256u * i) * VEC;
+            if (c < cols) {
+                src.template load<VEC>(row, c, v[i]);
+#pragma unroll
+                for (int j = 0; j < VEC; j++) { top = fmaxf(top, finite_abs(v[i][j])); sum[i][j] += v[i][j]; }
+            }
+        }
+        float scale = 1.0f;
+        if (out.exps) {
+            const int s = scale_for(block_max(top, red));
+            if (threadIdx.x == 0) out.exps[row] = s;
+            scale = pow2(s);
+        }
+        if (out.hi) {
+#pragma unroll
+            for (int i = 0; i < U; i++) {
+                const uint32_t c = (threadIdx.x + 256u * i) * VEC;
+                if (c < cols) put_planes<VEC>(out.hi + row * out.pitch + c, out.lo ? out.lo + row * out.pitch + c : nullptr, v[i], scale);
+            }
+        }
+    }
+    if (out.sums) {
+#pragma unroll
+        for (int i = 0; i < U; i++)
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+                const uint32_t c = (threadIdx.x + 256u * i) * VEC + j;
+                if (c < cols) out.sums[(uint64_t)blockIdx.x * cols + c] = sum[i][j];
+            }
+    }
+}
+// rows longer than a block's registers: the values are made twice, the sums by k_grad_sums
+template <class Src>
+__global__ void __launch_bounds__(256)
+k_split_long_rows(const Src src, const Planes out, uint32_t rows, uint32_t cols) {
+    __shared__ float red[8];
+    for (uint64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        float v[1], top = 0.0f;
+        for (uint32_t c = threadIdx.x; c < cols; c += 256) { src.template load<1>(row, c, v); top = fmaxf(top, finite_abs(v[0])); }
+        float scale = 1.0f;
+        if (out.exps) {
+            const int s = scale_for(block_max(top, red));
+            if (threadIdx.x == 0) out.exps[row] = s;
+            scale = pow2(s);
+        }
+        for (uint32_t c = threadIdx.x; c < cols; c += 256) {
+            src.template load<1>(row, c, v);
+            put_planes<1>(out.hi + row * out.pitch + c, out.lo ? out.lo + row * out.pitch + c : nullptr, v, scale);
+        }
+    }
+}
+template <class Src>
+__global__ void __launch_bounds__(256)
+k_grad_sums(const Src src, float *sums, uint32_t rows, uint32_t cols) {
+    const uint32_t c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= cols) return;
+    float v[1], s = 0.0f;
+    for (uint64_t row = blockIdx.y; row < rows; row += gridDim.y) { src.template load<1>(row, c, v); s += v[0]; }
+    sums[(uint64_t)blockIdx.y * cols + c] = s;
+}
+// sums[n][cols] -> out: 32 columns a block, eight threads a column, in block order
 template <typename T>
 __global__ void __launch_bounds__(256)
-k_col_sums(T *out, const float *dz, uint32_t M, uint32_t N) {
+k_fold_sums(T *out, const float *sums, uint32_t n, uint32_t cols) {
     __shared__ float red[8][33];
     const uint32_t c = blockIdx.x * 32 + (threadIdx.x & 31u), q = threadIdx.x >> 5;
     float s = 0.0f;
-    if (c < N) for (uint64_t m = q; m < M; m += 8) s += dz[m * N + c];
+    if (c < cols) for (uint32_t i = q; i < n; i += 8) s += sums[(uint64_t)i * cols + c];
     red[q][threadIdx.x & 31u] = s;
     __syncthreads();
-    if (q == 0 && c < N) {
+    if (q == 0 && c < cols) {
         s = 0.0f;
+#pragma unroll
         for (int i = 0; i < 8; i++) s += red[i][threadIdx.x];
         put_f32(out + c, s);
     }
 }
 
+// Scales by columns: the largest of x 2^-shift[row] over a run of rows, then the planes of it.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256)
+k_col_tops(const T *x, const int *shift, float *tops, uint32_t rows, uint32_t cols) {
+    const uint32_t c = (blockIdx.x * 256 + threadIdx.x) * VEC;
+    if (c >= cols) return;
+    float top[VEC] = {};
+    for (uint64_t row = blockIdx.y; row < rows; row += gridDim.y) {
+        float v[VEC];
+        load4<VEC>(x + row * cols + c, v);
+        const float f = pow2(-shift[row]);
+#pragma unroll
+        for (int j = 0; j < VEC; j++) top[j] = fmaxf(top[j], finite_abs(v[j] * f));
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; j++) tops[(uint64_t)blockIdx.y * cols + c + j] = top[j];
+}
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256)
+k_split_cols(const T *x, const int *shift, const float *tops, const Planes out, uint32_t rows, uint32_t cols) {
+    const uint32_t c = (blockIdx.x * 256 + threadIdx.x) * VEC;
+    if (c >= cols) return;
+    float scale[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; j++) {
+        float top = 0.0f;
+        for (uint32_t i = 0; i < gridDim.y; i++) top = fmaxf(top, tops[(uint64_t)i * cols + c + j]);
+        const int s = scale_for(top);
+        if (blockIdx.y == 0) out.exps[c + j] = s;
+        scale[j] = pow2(s);
+    }
+    for (uint64_t row = blockIdx.y; row < rows; row += gridDim.y) {
+        float v[VEC];
+        load4<VEC>(x + row * cols + c, v);
+        const float f = pow2(-shift[row]);
+#pragma unroll
+        for (int j = 0; j < VEC; j++) v[j] = v[j] * f * scale[j];
+        put_planes<VEC>(out.hi + row * out.pitch + c, out.lo ? out.lo + row * out.pitch + c : nullptr, v, 1.0f);
+    }
+}
+
+constexpr uint32_t ROW_VALUES = 8192;                  // a block of k_split_rows holds so many
+template <class Src>
+static void split_rows(const Src &src, const Planes &out, uint32_t rows, uint32_t cols, uint32_t blocks, const char *name) {
+    profile_begin();
+    if (cols > ROW_VALUES) {
+        if (out.hi) { k_split_long_rows<Src><<<grid_for(rows, 1, 8), 256, 0, g.stream>>>(src, out, rows, cols); after_launch(name); profile_begin(); }
+        if (out.sums) { k_grad_sums<Src><<<dim3((cols + 255) / 256, blocks), 256, 0, g.stream>>>(src, out.sums, rows, cols); after_launch(name); }
+        return;
+    }
+    if (cols % 4 == 0) {
+        if (cols <= 1024) k_split_rows<Src, 4, 1><<<blocks, 256, 0, g.stream>>>(src, out, rows, cols);
+        else if (cols <= 4096) k_split_rows<Src, 4, 4><<<blocks, 256, 0, g.stream>>>(src, out, rows, cols);
+        else k_split_rows<Src, 4, 8><<<blocks, 256, 0, g.stream>>>(src, out, rows, cols);
+    } else if (cols <= 1024) k_split_rows<Src, 1, 4><<<blocks, 256, 0, g.stream>>>(src, out, rows, cols);
+    else k_split_rows<Src, 1, 32><<<blocks, 256, 0, g.stream>>>(src, out, rows, cols);
+    after_launch(name);
+}
+static uint32_t split_blocks(uint32_t rows) { return grid_for(rows, 1, 6); }
+static uint32_t col_runs(uint32_t rows, uint32_t cols) {         // runs of rows that k_col_tops splits a column into
+    const uint32_t across = (cols + 1023) / 1024, most = (rows + 15) / 16;
+    uint32_t n = (uint32_t)g.sm_count * 4 / across;
+    if (n > 64) n = 64;
+    if (n > most) n = most;
+    return n ? n : 1;
+}
+
+// scratch of one call, cut into pieces
+struct Cut {
+    uint64_t at = 0;
+    uint8_t *base = nullptr;
+    template <typename T> T *take(uint64_t n) { T *p = (T *)(base + at); at += (n * sizeof(T) + 255) & ~255ull; return p; }
+};
+static Planes take_planes(Cut &c, uint32_t rows, uint32_t cols, bool lo, bool exps, uint32_t n_exps) {
+    Planes p{};
+    p.pitch = (cols + 7u) & ~7ull;
+    p.hi = c.take<__half>(rows * p.pitch);
+    p.lo = lo ? c.take<__half>(rows * p.pitch) : nullptr;
+    p.exps = exps ? c.take<int>(n_exps) : nullptr;
+    return p;
+}
+static hg::Operand operand(const Planes &p, bool mn) { return hg::Operand{p.hi, p.lo, p.pitch, mn}; }
+
+// ---- epilogue of a layer: out = act(sum 2^-exps + bias) + residual ----
+template <typename T> struct LayerEpi {
+    static constexpr bool mirrors = false;
+    T *out, *z; const T *bias, *residual; const int *row_exps, *col_exps; uint32_t act, N;
+    float bias_n; int exp_n;                           // of the lane's column
+    __device__ void column(uint32_t n) { bias_n = bias ? to_f32(bias[n]) : 0.0f; exp_n = col_exps ? col_exps[n] : 0; }
+    __device__ void mirror(uint32_t, uint32_t, float) const {}
+    __device__ void put(uint32_t m, uint32_t n, float v, uint32_t) const {
+        const int e = -(row_exps ? row_exps[m] : 0) - exp_n, h = e >> 1;       // up to 252 either way: two exact factors
+        v = v * pow2(h) * pow2(e - h) + bias_n;
+        const uint64_t at = (uint64_t)m * N + n;
+        if (z) put_f32(z + at, v);
+        v = act_value(act, v);
+        if (residual) v += to_f32(residual[at]);
+        put_f32(out + at, v);
+    }
+};
+
+// an f16 matrix as it is, or copied to a pitch that tile loads can take
+static hg::Operand f16_operand(Cut &c, const __half *p, uint32_t rows, uint32_t cols, bool mn, bool copy) {
+    if (cols % 8 == 0) return hg::Operand{p, nullptr, cols, mn};
+    const Planes q = take_planes(c, rows, cols, false, false, 0);
+    if (copy) split_rows(RowsOf<__half>{p, nullptr, cols}, q, rows, cols, split_blocks(rows), "layer_operand");
+    return operand(q, mn);
+}
+
 template <typename T>
 static void linear_forward(void *y, void *z, const void *x, const void *w, const void *bias, const void *residual, uint32_t M, uint32_t K, uint32_t N, uint32_t act) {
-    profile_begin();
-    product<T, T>(Strided{x, K, 1}, Strided{w, 1, N}, LinearEpi<T>{(T *)y, (T *)z, (const T *)bias, (const T *)residual, act, N}, M, N, K);
-    after_launch("linear");
+    constexpr bool F = sizeof(T) == 4;
+    const hg::Plan plan = hg::plan(M, N, K, true);
+    LayerEpi<T> epi{(T *)y, (T *)z, (const T *)bias, (const T *)residual, nullptr, nullptr, act, N, 0.0f, 0};
+    Cut c;
+    hg::Operand A{}, B{};
+    float *partial = nullptr;
+    for (int pass = 0; pass < 2; pass++) {             // the first pass measures
+        if (pass) { c.base = (uint8_t *)scratch_reserve(c.at); c.at = 0; }
+        partial = c.take<float>(plan.partial_bytes / 4);
+        if constexpr (F) {
+            const Planes pw = take_planes(c, K, N, true, true, K), px = take_planes(c, M, K, true, true, M);
+            A = operand(px, false); B = operand(pw, true);
+            epi.row_exps = px.exps;
+            if (pass) {
+                split_rows(RowsOf<float>{(const float *)w, nullptr, N}, pw, K, N, split_blocks(K), "layer_operand");
+                split_rows(RowsOf<float>{(const float *)x, pw.exps, K}, px, M, K, split_blocks(M), "layer_operand");
+            }
+        } else {
+            A = f16_operand(c, (const __half *)x, M, K, false, pass);
+            B = f16_operand(c, (const __half *)w, K, N, true, pass);
+        }
+    }
+    hg::product(A, B, M, N, K, plan, partial, epi, false, "linear");
 }
 
 template <typename T>
 static void linear_backward(void *dx, void *dw, void *dbias, const void *dy, const void *z, const void *x, const void *w, uint32_t M, uint32_t K, uint32_t N, uint32_t act) {
-    const uint64_t mn = (uint64_t)M * N;
-    float *dz = (float *)scratch_reserve(mn * 4);
-    profile_begin();
-    k_dz<T><<<grid_for(mn, 256, 8), 256, 0, g.stream>>>(dz, (const T *)dy, (const T *)z, act, mn);
-    after_launch("linear_backward_dz");
-    if (dbias) { k_col_sums<T><<<(N + 31) / 32, 256, 0, g.stream>>>((T *)dbias, dz, M, N); after_launch("linear_backward_bias"); }
-    if (dx) { product<float, T>(Strided{dz, N, 1}, Strided{w, N, 1}, PlainEpi<T>{(T *)dx, K}, M, K, N); after_launch("linear_backward_dx"); }
-    if (dw) { product<T, float>(Strided{x, 1, K}, Strided{dz, 1, N}, PlainEpi<T>{(T *)dw, N}, K, N, M); after_launch("linear_backward_dw"); }
+    constexpr bool F = sizeof(T) == 4;
+    const bool smooth = act == THC_ACT_GELU || act == THC_ACT_SILU;
+    const bool scaled = F || smooth;                   // dz needs planes: f32, or f16 times a slope that is neither 0 nor 1
+    const bool as_is = !F && act == THC_ACT_NONE && N % 8 == 0;
+    const GradOf<T> grad{(const T *)dy, (const T *)z, N, act};
+    const hg::Plan plan_x = hg::plan(M, K, N, true), plan_w = hg::plan(K, N, M, true);
+    const uint32_t blocks = split_blocks(M), sum_rows = N > ROW_VALUES ? (M < 16 ? M : 16) : blocks, runs = col_runs(M, K);
+    Cut c;
+    for (int pass = 0; pass < 2; pass++) {
+        if (pass) { c.base = (uint8_t *)scratch_reserve(c.at); c.at = 0; }
+        float *partial = c.take<float>((plan_x.partial_bytes > plan_w.partial_bytes ? plan_x.partial_bytes : plan_w.partial_bytes) / 4);
+        // dz, and its sums over rows
+        Planes pz{};
+        if (!as_is && (dx || dw)) pz = take_planes(c, M, N, scaled, scaled, M);
+        pz.sums = dbias ? c.take<float>((uint64_t)sum_rows * N) : nullptr;
+        if (pass && (pz.hi || pz.sums)) split_rows(grad, pz, M, N, N > ROW_VALUES && pz.sums ? sum_rows : blocks, "linear_backward_dz");
+        if (pass && dbias) {
+            profile_begin();
+            k_fold_sums<T><<<(N + 31) / 32, 256, 0, g.stream>>>((T *)dbias, pz.sums, sum_rows, N);
+            after_launch("linear_backward_bias");
+        }
+        const hg::Operand dz_k = as_is ? hg::Operand{(const __half *)dy, nullptr, N, false} : operand(pz, false);
+        hg::Operand dz_mn = dz_k;
+        dz_mn.mn = true;
+        if (dx) {
+            LayerEpi<T> epi{(T *)dx, nullptr, nullptr, nullptr, pz.exps, nullptr, THC_ACT_NONE, K, 0.0f, 0};
+            hg::Operand W{};
+            if constexpr (F) {
+                const Planes pw = take_planes(c, K, N, true, true, K);
+                if (pass) split_rows(RowsOf<float>{(const float *)w, nullptr, N}, pw, K, N, split_blocks(K), "layer_operand");
+                W = operand(pw, false);
+                epi.col_exps = pw.exps;
+            } else W = f16_operand(c, (const __half *)w, K, N, false, pass);
+            if (pass) hg::product(dz_k, W, M, K, N, plan_x, partial, epi, false, "linear_backward_dx");
+        }
+        if (dw) {
+            LayerEpi<T> epi{(T *)dw, nullptr, nullptr, nullptr, nullptr, nullptr, THC_ACT_NONE, N, 0.0f, 0};
+            hg::Operand X{};
+            if (scaled) {                              // x takes dz's scales back
+                const Planes px = take_planes(c, M, K, F, true, K);
+                float *tops = c.take<float>((uint64_t)runs * K);
+                if (pass) {
+                    profile_begin();
+                    const T *xs = (const T *)x;
+                    if (K % 4 == 0) {
+                        k_col_tops<T, 4><<<dim3((K / 4 + 255) / 256, runs), 256, 0, g.stream>>>(xs, pz.exps, tops, M, K);
+                        k_split_cols<T, 4><<<dim3((K / 4 + 255) / 256, runs), 256, 0, g.stream>>>(xs, pz.exps, tops, px, M, K);
+                    } else {
+                        k_col_tops<T, 1><<<dim3((K + 255) / 256, runs), 256, 0, g.stream>>>(xs, pz.exps, tops, M, K);
+                        k_split_cols<T, 1><<<dim3((K + 255) / 256, runs), 256, 0, g.stream>>>(xs, pz.exps, tops, px, M, K);
+                    }
+                    after_launch("layer_operand");
+                }
+                X = operand(px, true);
+                epi.row_exps = px.exps;
+            } else if constexpr (!F) X = f16_operand(c, (const __half *)x, M, K, true, pass);
+            if (pass) hg::product(X, dz_mn, K, N, M, plan_w, partial, epi, false, "linear_backward_dw");
+        }
+    }
 }
 
 static bool linear_shape(const char *who, uint32_t M, uint32_t K, uint32_t N, uint32_t act, uint32_t dtype) {
