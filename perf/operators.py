@@ -139,22 +139,25 @@ EPS = 1e-5
 LR, MU, DECAY = 0.02, 0.95, 0.01
 
 
-class _Pointer:
-    def __init__(self, ptr, shape, kind):
-        self.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": kind, "data": (ptr, False), "version": 3}
-
-
-class Buf:
-    """A buffer of the library's pool, and the tensor that lies in it."""
+class _Memory:
+    """A buffer of the library's pool; tensors that lie in it keep it alive."""
 
     def __init__(self, shape, dtype):
-        self.lib = _backend().lib
-        n = math.prod(shape) * (2 if dtype is torch.float16 else 4)
-        self.id = _backend().alloc(max(n, 512))
-        self.t = torch.as_tensor(_Pointer(self.lib.thvm_cuda_buf_ptr(self.id), shape, "<f2" if dtype is torch.float16 else "<f4"), device="cuda")
+        be = _backend()
+        size = 2 if dtype is torch.float16 else 4
+        self.lib, self.id = be.lib, be.alloc(max(math.prod(shape) * size, 512))
+        self.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": "<f%d" % size, "data": (self.lib.thvm_cuda_buf_ptr(self.id), False), "version": 3}
 
     def __del__(self):
         self.lib.thvm_cuda_buf_free(self.id)
+
+
+class Buf:
+    """A buffer's id, and the tensor that lies in it."""
+
+    def __init__(self, shape, dtype):
+        memory = _Memory(shape, dtype)
+        self.id, self.t = memory.id, torch.as_tensor(memory, device="cuda")
 
 
 _be = None
@@ -187,16 +190,13 @@ def _outputs(case):
 def prepare(case, seed):
     state = {"case": case, "t": _inputs(case, seed)}
     if own:
-        lib = _backend().lib
-        state["lib"], state["b"] = lib, {}
+        lib = state["lib"] = _backend().lib
+        b = state["b"] = {name: Buf(t.shape, t.dtype) for name, t in state["t"].items()}
+        b.update({name: Buf(shape, dt) for name, shape, dt in _outputs(case)})
+        lib.thvm_cuda_sync()            # fresh buffers are cleared on the library's stream
         for name, t in state["t"].items():
-            b = state["b"][name] = Buf(t.shape, t.dtype)
-            lib.thvm_cuda_sync()
-            b.t.copy_(t)
-            state["t"][name] = b.t
-        for name, shape, dt in _outputs(case):
-            state["b"][name] = Buf(shape, dt)
-        lib.thvm_cuda_sync()
+            b[name].t.copy_(t)
+        state["t"] = None
         torch.cuda.synchronize()
     return state
 
