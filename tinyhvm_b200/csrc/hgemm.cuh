@@ -14,7 +14,8 @@
 // two accumulators.  Within a block of k the small products go first.
 //
 // A CTA pair (cta_group::2) computes a 256 x NT tile, NT = 256 or 128: each CTA holds 128 rows of A, half of B's
-// columns, and the accumulators of its own rows.  Roles: warps 0-7 epilogue, warp 8 tile loads, warp 9 (first CTA) MMAs.  The pairs are
+// columns, and the accumulators of its own rows.  Roles: warps 0-7 epilogue, warps 8 and 9 tile loads of A and of B, warp 10
+// (first CTA) MMAs; 11 fills up their warpgroup.  The pairs are
 // persistent and walk over the tiles, so the next tile's loads and MMAs run under this one's epilogue.
 //
 // Operands may lie either way round, as the matrix descriptors allow for f16: k along memory rows (boxes of 64 k x rows),
@@ -32,13 +33,19 @@
 namespace thc {
 namespace hg {
 
-constexpr uint32_t EPI_WARPS = 8, TMA_WARP = 8, MMA_WARP = 9, THREADS = 320;
+constexpr uint32_t EPI_WARPS = 8, TMA_A_WARP = 8, TMA_B_WARP = 9, MMA_WARP = 10, THREADS = 384;
+// 168 registers a thread at launch (65536 / 384, by eights); the epilogue's two warpgroups take from the third: 128 x 40 + 256 x 232 = 384 x 168
+constexpr uint32_t EPI_REGS = 232, IO_REGS = 40;
 constexpr uint32_t KB = 64;                                // k of a block: 128 bytes, the swizzle's width
 constexpr uint32_t A_PLANE = 128 * 128;                    // bytes of one CTA's A plane of a block
 constexpr uint32_t RING_BYTES = 196608, STAGING = EPI_WARPS * 4096;
 constexpr uint32_t MAX_STAGES = 8;
 constexpr uint32_t WAIT_LIMIT = 1u << 24;
 constexpr int STATUS_TIMEOUT = 8;
+// How an operand lies in memory, and its tile loads: k along rows, [planes][rows][k]; m / n along rows whose pitch is a multiple of 64,
+// seen as [planes][blocks of 64][k][64]; or the latter with one plane and any pitch, a load per block.  (A load costs
+// the issuing thread some 200 cycles: with one per plane and block the loads, not the MMAs, set the pace.)
+enum : uint32_t { K_ROWS = 0, MN_BLOCKS = 1, MN_BOXES = 2 };
 
 struct Shared {
     unsigned long long full[MAX_STAGES], empty[MAX_STAGES], acc_full[2], acc_empty[2];
@@ -53,10 +60,10 @@ struct Shape {
     uint32_t blocks, split_blocks, chunk;                  // blocks of 64 k: in all, per split, per chunk
     uint32_t splits;
     uint32_t stages, stage_bytes, a_bytes;
-    uint32_t a_mn, b_mn, a_lo, b_lo, upper;
+    uint32_t a_mode, b_mode, a_lo, b_lo, upper;
     int *status;
 };
-struct Maps { CUtensorMap a[2], b[2]; };
+struct Maps { CUtensorMap a, b; };
 
 // ---- PTX ----
 __device__ __forceinline__ uint32_t smem32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -67,13 +74,13 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(n) : "memory"); }
-__device__ __forceinline__ void bar_arrive(uint32_t cluster_addr) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory"); }
+__device__ __forceinline__ void bar_arrive(uint32_t cluster_addr) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory"); }
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
 // false after WAIT_LIMIT polls or when another thread of this CTA gave up
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
     for (uint32_t it = 0; it < WAIT_LIMIT; ++it) {
         uint32_t ok;
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
         if (ok) return true;
         if ((it & 255u) == 255u && *abort_flag) return false;
@@ -81,10 +88,20 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
     *abort_flag = 1;
     return false;
 }
-// box at (x, y) of the map into this CTA's shared memory, signalled on a barrier of the pair's first CTA
-__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, uint32_t bar, uint32_t x, uint32_t y) {
-    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                 ::"r"(dst), "l"(map), "r"(bar), "r"((int)x), "r"((int)y) : "memory");
+// a box of the map into this CTA's shared memory, signalled on a barrier of the pair's first CTA
+__device__ __forceinline__ void load_box3(uint32_t dst, const CUtensorMap *map, uint32_t bar, uint32_t x, uint32_t y) {
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"((int)x), "r"((int)y), "r"(0) : "memory");
+}
+__device__ __forceinline__ void load_box4(uint32_t dst, const CUtensorMap *map, uint32_t bar, uint32_t y, uint32_t z) {
+    asm volatile("cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(0), "r"((int)y), "r"((int)z), "r"(0) : "memory");
+}
+// One operand's tile of a block of k: all its planes, `blocks` x 64 of m / n where they run along memory rows.
+__device__ __forceinline__ void load_operand(uint32_t dst, const CUtensorMap *map, uint32_t bar, uint32_t mode, uint32_t blocks, uint32_t mn, uint32_t k) {
+    if (mode == K_ROWS) load_box3(dst, map, bar, k, mn);
+    else if (mode == MN_BLOCKS) load_box4(dst, map, bar, k, mn / 64u);
+    else for (uint32_t j = 0; j < blocks; j++) load_box3(dst + j * 8192u, map, bar, mn + j * 64u, k);
 }
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
@@ -136,8 +153,75 @@ template <uint32_t NT> __device__ __forceinline__ Tile tile_of(const Shape &S, u
     return r;
 }
 
-// Epi: what happens to a finished sum.  put(m, n, v, z) is called with n running along the lanes; with Epi::mirror,
-// mirror(n, m, v) too, m running along the lanes, for the transposed place of a symmetric product.
+// Epi: what happens to finished sums, R rows (m, m + step, ...; those below M count) of V neighbouring columns at a time (V = 4 where
+// Epi::wide() says that the result's rows allow it, else 1).  column<V>(n) sets up what belongs to the columns n, n+1, ...; fetch<V>(m, n, x)
+// reads what a row's result needs from memory; put<V, R>(rows, n, v, x, z) finishes and stores.  With Epi::mirrors, mirror<V, R> stores
+// the transposed place of a symmetric product: rows along n, V neighbouring values of m.
+struct Rows { uint32_t first, step, end; };
+
+// A block of 32 x 32 sums passes through shared memory, one warp's 4 KB, from "a lane holds a row" to "eight lanes hold a row" (or
+// 32 lanes, V = 1).  16-byte chunk c of row r lies at chunk c ^ swap(r): whole rows, rows by chunk and columns by four are all read
+// and written without bank conflicts.
+//
+// Four rows of a lane go together, so that every choice the epilogue makes is one branch for all of them and their arithmetic
+// overlaps: two warps a scheduler hide no latency (row by row, a tile's epilogue took 18000 cycles; the MMAs of K = 1024 take 8000).
+__device__ __forceinline__ uint32_t swap(uint32_t r) { return (r ^ (r >> 2)) & 7u; }
+template <int V, class Epi>
+__device__ __forceinline__ void put_block(Epi &e, const float *st, uint32_t lane, uint32_t m0, uint32_t n0, uint32_t M, uint32_t N, uint32_t z) {
+    constexpr uint32_t STEP = V == 4 ? 4 : 1;
+    const uint32_t ro = V == 4 ? lane >> 3 : 0u, n = n0 + (V == 4 ? (lane & 7u) * 4u : lane);
+    if (n >= N) return;
+    e.template column<V>(n);
+#pragma unroll 1
+    for (uint32_t r0 = ro; r0 < 32u; r0 += 4 * STEP) {
+        float x[4][V], v[4][V];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++)
+            if (m0 + r0 + i * STEP < M) e.template fetch<V>(m0 + r0 + i * STEP, n, x[i]);
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            const uint32_t r = r0 + i * STEP;
+            if constexpr (V == 4) {
+                const float4 q = *reinterpret_cast<const float4 *>(st + r * 32u + (((lane & 7u) ^ swap(r)) << 2));
+                v[i][0] = q.x; v[i][1] = q.y; v[i][2] = q.z; v[i][3] = q.w;
+            } else v[i][0] = st[r * 32u + (((lane >> 2) ^ swap(r)) << 2) + (lane & 3u)];
+        }
+        e.template put<V, 4>(Rows{m0 + r0, STEP, M}, n, v, x, z);
+    }
+}
+template <int V, class Epi>
+__device__ __forceinline__ void mirror_block(Epi &e, const float *st, uint32_t lane, uint32_t m0, uint32_t n0, uint32_t N) {
+    constexpr uint32_t STEP = V == 4 ? 4 : 1;
+    const uint32_t no = V == 4 ? lane >> 3 : 0u, mo = V == 4 ? (lane & 7u) * 4u : lane;
+#pragma unroll 1
+    for (uint32_t c0 = no; c0 < 32u; c0 += 4 * STEP) {
+        float v[4][V];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            const uint32_t c = c0 + i * STEP;
+#pragma unroll
+            for (uint32_t j = 0; j < V; j++) v[i][j] = st[(mo + j) * 32u + (((c >> 2) ^ swap(mo + j)) << 2) + (c & 3u)];
+        }
+        e.template mirror<V, 4>(Rows{n0 + c0, STEP, N}, m0 + mo, v);
+    }
+}
+// a block on the diagonal: each value decides for itself
+template <class Epi>
+__device__ __forceinline__ void diagonal_block(Epi &e, const float *st, uint32_t lane, uint32_t m0, uint32_t n0, uint32_t M, uint32_t N) {
+    const uint32_t n = n0 + lane;
+    if (n >= N) return;
+#pragma unroll 1
+    for (uint32_t r = 0; r < 32u; r++) {
+        const uint32_t m = m0 + r;
+        if (m > n || m >= M) break;
+        const float s = st[r * 32u + (((lane >> 2) ^ swap(r)) << 2) + (lane & 3u)];
+        float x[1][1], v[1][1] = {{s}}, w[1][1] = {{s}};
+        e.template fetch<1>(m, n, x[0]);
+        e.template put<1, 1>(Rows{m, 1, M}, n, v, x, 0);
+        if (m < n) e.template mirror<1, 1>(Rows{n, 1, N}, m, w);
+    }
+}
+
 template <uint32_t NT, class Epi>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 k_hgemm(const __grid_constant__ Shape S, const __grid_constant__ Maps maps, const __grid_constant__ Epi epi) {
@@ -166,12 +250,15 @@ k_hgemm(const __grid_constant__ Shape S, const __grid_constant__ Maps maps, cons
     const uint32_t ring = smem32(base);
     constexpr uint32_t B_PLANE = NT / 2 * 128;             // bytes of this CTA's B plane of a block
 
+    if (warp < EPI_WARPS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(EPI_REGS));
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(IO_REGS));
     if (warp < EPI_WARPS) {
         // ================= epilogue: rows of this CTA, quadrant warp % 4; columns half warp / 4 =================
         constexpr uint32_t COLS = NT / 2;
         const uint32_t q = warp & 3u, half = warp >> 2;
         float *st = reinterpret_cast<float *>(base + RING_BYTES) + warp * 1024u;
-        Epi e = epi;                                       // (keeps what belongs to the lane's column)
+        Epi e = epi;                                       // (keeps what belongs to the lane's columns)
+        const bool wide = e.wide();
         bool ok = true;
         uint32_t c = 0;                                    // chunks so far
         for (uint32_t t = pair; t < S.tiles && ok; t += pairs) {
@@ -198,58 +285,50 @@ k_hgemm(const __grid_constant__ Shape S, const __grid_constant__ Maps maps, cons
             }
             if (!ok) break;
             const uint32_t m0 = T.m0 + rank * 128u + q * 32u, n0 = T.n0 + half * COLS;
-#pragma unroll
+#pragma unroll 1
             for (uint32_t j = 0; j < COLS / 32; j++) {
                 const uint32_t n1 = n0 + j * 32u;
-                if (n1 >= S.N || m0 >= S.M) continue;
+                if (n1 >= S.N || m0 >= S.M) break;
+                __syncwarp();
+#pragma unroll
+                for (uint32_t k = 0; k < COLS / 32; k++)           // (registers are picked by number, not by index)
+                    if (k == j) {
+#pragma unroll
+                        for (uint32_t i = 0; i < 8; i++)
+                            *reinterpret_cast<float4 *>(st + lane * 32u + ((i ^ swap(lane)) << 2)) = make_float4(acc[k * 32 + 4 * i], acc[k * 32 + 4 * i + 1], acc[k * 32 + 4 * i + 2], acc[k * 32 + 4 * i + 3]);
+                    }
+                __syncwarp();
+                bool above = false;
                 if constexpr (Epi::mirrors) {
                     if (S.upper) {
-#pragma unroll
-                        for (uint32_t i = 0; i < 32; i++)  // this thread's row m0 + lane: neighbours in the transposed row
-                            if (m0 + lane < n1 + i && n1 + i < S.N) e.mirror(n1 + i, m0 + lane, acc[j * 32 + i]);
+                        if (n1 + 31u < m0) continue;
+                        if (n1 <= m0 + 31u) { diagonal_block(e, st, lane, m0, n1, S.M, S.N); continue; }
+                        above = true;
                     }
                 }
-                __syncwarp();
-#pragma unroll
-                for (uint32_t i = 0; i < 32; i++) st[lane * 32u + (i ^ lane)] = acc[j * 32 + i];
-                __syncwarp();
-                const uint32_t n = n1 + lane;
-                const uint32_t rows = S.M - m0 < 32u ? S.M - m0 : 32u;
-                if (n < S.N) {
-                    e.column(n);
-#pragma unroll 4
-                    for (uint32_t r = 0; r < rows; r++) {
-                        const float v = st[r * 32u + (lane ^ r)];
-                        if (!(Epi::mirrors && S.upper && m0 + r > n)) e.put(m0 + r, n, v, T.z);
-                    }
+                if (wide) put_block<4>(e, st, lane, m0, n1, S.M, S.N, T.z);
+                else put_block<1>(e, st, lane, m0, n1, S.M, S.N, T.z);
+                if constexpr (Epi::mirrors) {
+                    if (above) { if (wide) mirror_block<4>(e, st, lane, m0, n1, S.N); else mirror_block<1>(e, st, lane, m0, n1, S.N); }
                 }
             }
         }
-    } else if (warp == TMA_WARP) {
-        // ================= tile loads: one thread per CTA =================
+    } else if (warp == TMA_A_WARP || warp == TMA_B_WARP) {
+        // ================= tile loads: one thread per CTA and operand =================
         if (lane == 0) {
+            const bool is_a = warp == TMA_A_WARP;
+            const CUtensorMap *map = is_a ? &maps.a : &maps.b;
+            const uint32_t mode = is_a ? S.a_mode : S.b_mode, boxes = is_a ? 2u : NT / 128, width = is_a ? 128u : NT / 2, at = is_a ? 0u : S.a_bytes;
             bool ok = true;
             uint32_t it = 0, s = 0, use = 0;
-            const uint32_t planes_a = 1u + S.a_lo, planes_b = 1u + S.b_lo;
             for (uint32_t t = pair; t < S.tiles && ok; t += pairs) {
                 const Tile T = tile_of<NT>(S, t);
-                const uint32_t m = T.m0 + rank * 128u, n = T.n0 + rank * (NT / 2);
+                const uint32_t mn = (is_a ? T.m0 : T.n0) + rank * width;
                 for (uint32_t kb = 0; kb < T.blocks; kb++) {
                     if (use) ok = bar_wait(smem32(&sh.empty[s]), (use - 1) & 1u, abort_flag);
                     if (!ok) break;
-                    const uint32_t bar = in_cta(smem32(&sh.full[s]), 0), k = (T.block0 + kb) * KB;
-                    if (rank == 0) bar_expect(smem32(&sh.full[s]), 2u * S.stage_bytes);
-                    uint32_t dst = ring + s * S.stage_bytes;
-                    for (uint32_t p = 0; p < planes_a; p++, dst += A_PLANE) {
-                        if (S.a_mn) { load_box(dst, &maps.a[p], bar, m, k); load_box(dst + 8192u, &maps.a[p], bar, m + 64u, k); }
-                        else load_box(dst, &maps.a[p], bar, k, m);
-                    }
-                    for (uint32_t p = 0; p < planes_b; p++, dst += B_PLANE) {
-                        if (S.b_mn) {
-#pragma unroll
-                            for (uint32_t j = 0; j < NT / 128; j++) load_box(dst + j * 8192u, &maps.b[p], bar, n + j * 64u, k);
-                        } else load_box(dst, &maps.b[p], bar, k, n);
-                    }
+                    if (is_a && rank == 0) bar_expect(smem32(&sh.full[s]), 2u * S.stage_bytes);
+                    load_operand(ring + s * S.stage_bytes + at, map, in_cta(smem32(&sh.full[s]), 0), mode, boxes, mn, (T.block0 + kb) * KB);
                     it++;
                     if (++s == S.stages) { s = 0; use++; }
                 }
@@ -262,11 +341,12 @@ k_hgemm(const __grid_constant__ Shape S, const __grid_constant__ Maps maps, cons
             }
         }
         __syncwarp();
-    } else if (rank == 0) {
+    } else if (warp == MMA_WARP && rank == 0) {
         // ================= MMAs: one thread, for the pair =================
         if (lane == 0) {
-            const uint32_t idesc = (1u << 4) | (S.a_mn << 15) | (S.b_mn << 16) | ((NT >> 3) << 17) | ((256u >> 4) << 24);   // f32 sums of f16 products
-            const uint64_t step_a = S.a_mn ? 2048u >> 4 : 32u >> 4, step_b = S.b_mn ? 2048u >> 4 : 32u >> 4;                 // 16 k further
+            const uint32_t a_mn = S.a_mode != K_ROWS, b_mn = S.b_mode != K_ROWS;
+            const uint32_t idesc = (1u << 4) | (a_mn << 15) | (b_mn << 16) | ((NT >> 3) << 17) | ((256u >> 4) << 24);   // f32 sums of f16 products
+            const uint64_t step_a = a_mn ? 2048u >> 4 : 32u >> 4, step_b = b_mn ? 2048u >> 4 : 32u >> 4;                 // 16 k further
             bool ok = true;
             uint32_t s = 0, use = 0, c = 0;
             for (uint32_t t = pair; t < S.tiles && ok; t += pairs) {
@@ -281,14 +361,14 @@ k_hgemm(const __grid_constant__ Shape S, const __grid_constant__ Maps maps, cons
                         if (!ok) break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         const uint32_t sa = ring + s * S.stage_bytes, sb = sa + S.a_bytes;
-                        const uint64_t a_hi = operand_desc(sa, S.a_mn), b_hi = operand_desc(sb, S.b_mn);
+                        const uint64_t a_hi = operand_desc(sa, a_mn), b_hi = operand_desc(sb, b_mn);
                         if (S.a_lo) {
-                            const uint64_t a_lo = operand_desc(sa + A_PLANE, S.a_mn);
+                            const uint64_t a_lo = operand_desc(sa + A_PLANE, a_mn);
 #pragma unroll
                             for (uint32_t k = 0; k < 4; k++) { mma(d, a_lo + k * step_a, b_hi + k * step_b, idesc, more); more = 1; }
                         }
                         if (S.b_lo) {
-                            const uint64_t b_lo = operand_desc(sb + B_PLANE, S.b_mn);
+                            const uint64_t b_lo = operand_desc(sb + B_PLANE, b_mn);
 #pragma unroll
                             for (uint32_t k = 0; k < 4; k++) { mma(d, a_hi + k * step_a, b_lo + k * step_b, idesc, more); more = 1; }
                         }
@@ -318,32 +398,45 @@ k_hgemm(const __grid_constant__ Shape S, const __grid_constant__ Maps maps, cons
 struct PartialEpi {
     static constexpr bool mirrors = false;
     float *partial; uint64_t mn; uint32_t N;
-    __device__ void column(uint32_t) const {}
-    __device__ void mirror(uint32_t, uint32_t, float) const {}
-    __device__ void put(uint32_t m, uint32_t n, float v, uint32_t z) const { partial[z * mn + (uint64_t)m * N + n] = v; }
+    __device__ bool wide() const { return N % 4 == 0; }
+    template <int V> __device__ void column(uint32_t) const {}
+    template <int V> __device__ void fetch(uint32_t, uint32_t, float (&)[V]) const {}
+    template <int V, int R> __device__ void put(Rows r, uint32_t n, const float (&v)[R][V], const float (&)[R][V], uint32_t z) const {
+#pragma unroll
+        for (uint32_t i = 0; i < R; i++) if (r.first + i * r.step < r.end) store_vec<V>(partial + z * mn + (uint64_t)(r.first + i * r.step) * N + n, v[i]);
+    }
 };
-template <class Epi>
+template <int V, class Epi>
 __global__ void __launch_bounds__(256)
 k_hgemm_fold(const float *partial, uint32_t splits, uint32_t M, uint32_t N, const __grid_constant__ Epi epi) {
-    const uint32_t n = blockIdx.x * 128 + (threadIdx.x & 127u);
+    const uint32_t n = (blockIdx.x * 32 + (threadIdx.x & 31u)) * V;
     if (n >= N) return;
     Epi e = epi;
-    e.column(n);
-    for (uint32_t m = blockIdx.y * 2 + (threadIdx.x >> 7); m < M; m += gridDim.y * 2) {
-        float v = 0.0f;
-        for (uint32_t z = 0; z < splits; z++) v += partial[((uint64_t)z * M + m) * N + n];
-        e.put(m, n, v, 0);
+    e.template column<V>(n);
+    for (uint32_t m = blockIdx.y * 8 + (threadIdx.x >> 5); m < M; m += gridDim.y * 8) {
+        float v[1][V], x[1][V];
+        e.template fetch<V>(m, n, x[0]);
+        load_vec<V>(partial + (uint64_t)m * N + n, v[0]);
+        for (uint32_t z = 1; z < splits; z++) {
+            float p[V];
+            load_vec<V>(partial + ((uint64_t)z * M + m) * N + n, p);
+#pragma unroll
+            for (int j = 0; j < V; j++) v[0][j] += p[j];
+        }
+        e.template put<V, 1>(Rows{m, 1, M}, n, v, x, 0);
     }
 }
 
 // ---- host ----
-// One operand: `rows` x `cols` f16 planes in memory, rows `pitch` values apart (a multiple of 8, base 16-byte aligned).  mn: the rows run
-// along k; otherwise along the operand's m or n.
-struct Operand { const __half *hi, *lo; uint64_t pitch; bool mn; };
+// One operand: one or two f16 planes of rows `pitch` values apart (a multiple of 8; base 16-byte aligned), the second `plane` values
+// behind the first (0: there is none).  mn: the rows run along the operand's m or n, one row per k, and with two planes the pitch is
+// a multiple of 64 and all of it may be read; otherwise along k.
+struct Operand { const __half *p; uint64_t pitch, plane; bool mn; };
 
 typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
                                 CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-static void make_map(CUtensorMap *m, const __half *base, uint64_t inner, uint64_t outer, uint64_t pitch, uint32_t box_outer) {
+// the operand's map and mode; rows: its m or n
+static uint32_t operand_map(CUtensorMap *m, const Operand &o, uint32_t rows, uint32_t K, uint32_t tile_rows) {
     static EncodeTiled fn = nullptr;
     if (!fn) {
         void *p = nullptr;
@@ -352,18 +445,24 @@ static void make_map(CUtensorMap *m, const __half *base, uint64_t inner, uint64_
         if (q != cudaDriverEntryPointSuccess) fatal("cuTensorMapEncodeTiled is not in this driver");
         fn = (EncodeTiled)p;
     }
-    const cuuint64_t dims[2] = {inner, outer}, strides[1] = {pitch * 2};
-    const cuuint32_t box[2] = {64, box_outer}, one[2] = {1, 1};
-    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<__half *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) fatal("tensor map of %llu x %llu values, pitch %llu: error %d", (unsigned long long)outer, (unsigned long long)inner, (unsigned long long)pitch, (int)r);
-}
-static void operand_maps(CUtensorMap (&maps)[2], const Operand &o, uint32_t rows, uint32_t K, uint32_t box_rows) {
-    for (int p = 0; p < 2; p++) {
-        const __half *base = p && o.lo ? o.lo : o.hi;
-        if (o.mn) make_map(&maps[p], base, rows, K, o.pitch, KB);
-        else make_map(&maps[p], base, K, rows, o.pitch, box_rows);
+    const uint32_t mode = !o.mn ? K_ROWS : o.pitch % 64 == 0 && (o.plane || rows % 64 == 0) ? MN_BLOCKS : MN_BOXES;
+    const cuuint64_t planes = o.plane ? 2 : 1, pitch = o.pitch * 2, plane = o.plane ? o.plane * 2 : pitch;
+    cuuint64_t dims[4], strides[3];
+    cuuint32_t box[4];
+    const cuuint32_t one[4] = {1, 1, 1, 1};
+    if (mode == MN_BLOCKS) {
+        dims[0] = 64; dims[1] = K; dims[2] = (rows + 63) / 64; dims[3] = planes;
+        strides[0] = pitch; strides[1] = 128; strides[2] = plane;
+        box[0] = 64; box[1] = KB; box[2] = tile_rows / 64; box[3] = (cuuint32_t)planes;
+    } else {
+        dims[0] = mode == K_ROWS ? K : rows; dims[1] = mode == K_ROWS ? rows : K; dims[2] = planes;
+        strides[0] = pitch; strides[1] = plane;
+        box[0] = 64; box[1] = mode == K_ROWS ? tile_rows : KB; box[2] = (cuuint32_t)planes;
     }
+    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, mode == MN_BLOCKS ? 4 : 3, const_cast<__half *>(o.p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) fatal("tensor map of %u x %u values, pitch %llu: error %d", rows, K, (unsigned long long)o.pitch, (int)r);
+    return mode;
 }
 
 struct Plan { uint32_t nt, splits; uint64_t partial_bytes; };
@@ -405,7 +504,7 @@ static void product(const Operand &A, const Operand &B, uint32_t M, uint32_t N, 
     S.blocks = (K + KB - 1) / KB;
     S.split_blocks = (S.blocks + p.splits - 1) / p.splits;
     S.splits = p.splits;
-    S.a_mn = A.mn; S.b_mn = B.mn; S.a_lo = A.lo != nullptr; S.b_lo = B.lo != nullptr;
+    S.a_lo = A.plane != 0; S.b_lo = B.plane != 0;
     S.chunk = S.a_lo || S.b_lo ? 2 : 8;
     S.a_bytes = A_PLANE * (1 + S.a_lo);
     S.stage_bytes = S.a_bytes + p.nt / 2 * 128 * (1 + S.b_lo);
@@ -416,16 +515,19 @@ static void product(const Operand &A, const Operand &B, uint32_t M, uint32_t N, 
     if (upper) { S.tiles = 0; for (uint32_t r = 0; r < S.row_tiles; r++) S.tiles += S.col_tiles - r * 256 / p.nt; }
     S.status = g.dev_status;
     Maps maps;
-    operand_maps(maps.a, A, M, K, 128);
-    operand_maps(maps.b, B, N, K, p.nt / 2);
-    if (p.splits > 1) {
+    S.a_mode = operand_map(&maps.a, A, M, K, 128);
+    S.b_mode = operand_map(&maps.b, B, N, K, p.nt / 2);
+    if constexpr (!Epi::mirrors) if (p.splits > 1) {
         const PartialEpi pe{partial, (uint64_t)M * N, N};
         if (p.nt == 256) launch<256>(S, maps, pe, name); else launch<128>(S, maps, pe, name);
         profile_begin();
-        k_hgemm_fold<Epi><<<dim3((N + 127) / 128, (M + 7) / 8 < 4096 ? (M + 7) / 8 : 4096), 256, 0, g.stream>>>(partial, p.splits, M, N, epi);
+        const uint32_t down = (M + 7) / 8 < 4096 ? (M + 7) / 8 : 4096;
+        if (N % 4 == 0) k_hgemm_fold<4, Epi><<<dim3((N + 127) / 128, down), 256, 0, g.stream>>>(partial, p.splits, M, N, epi);
+        else k_hgemm_fold<1, Epi><<<dim3((N + 31) / 32, down), 256, 0, g.stream>>>(partial, p.splits, M, N, epi);
         after_launch("layer_fold");
-    } else if (p.nt == 256) launch<256>(S, maps, epi, name);
-    else launch<128>(S, maps, epi, name);
+        return;
+    }
+    if (p.nt == 256) launch<256>(S, maps, epi, name); else launch<128>(S, maps, epi, name);
 }
 
 }  // namespace hg

@@ -19,7 +19,7 @@ __device__ __forceinline__ void put_f32(__half *p, float v) { *p = __float2half_
 // 16 bytes hold this many values
 template <typename T> struct Vec16 { static constexpr int n = 16 / (int)sizeof(T); };
 
-// V neighbouring values; V is 1 or Vec16<T>::n (p then 16-byte aligned)
+// V neighbouring values; p is aligned to V of them
 template <int V> __device__ __forceinline__ void load_vec(const float *p, float (&v)[V]) {
     if constexpr (V == 4) { const float4 q = *reinterpret_cast<const float4 *>(p); v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w; }
     else { v[0] = *p; }
@@ -30,6 +30,10 @@ template <int V> __device__ __forceinline__ void load_vec(const __half *p, float
         const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
         for (int i = 0; i < 4; i++) { const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i])); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
+    } else if constexpr (V == 4) {
+        const uint2 q = *reinterpret_cast<const uint2 *>(p);
+        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&q.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&q.y));
+        v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
     } else { v[0] = __half2float(*p); }
 }
 template <int V> __device__ __forceinline__ void store_vec(float *p, const float (&v)[V]) {
@@ -42,7 +46,18 @@ template <int V> __device__ __forceinline__ void store_vec(__half *p, const floa
 #pragma unroll
         for (int i = 0; i < 4; i++) { const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]); w[i] = *reinterpret_cast<const uint32_t *>(&h); }
         *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else if constexpr (V == 4) {
+        const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+        *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
     } else { *p = __float2half_rn(v[0]); }
+}
+// hi = f16(x), lo = f16(x - hi): the planes of V neighbouring values (hgemm.cuh)
+template <int V> __device__ __forceinline__ void store_planes(__half *hi, __half *lo, const float (&x)[V]) {
+    float h[V], l[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) { h[j] = __half2float(__float2half_rn(x[j])); l[j] = x[j] - h[j]; }
+    store_vec<V>(hi, h);
+    if (lo) store_vec<V>(lo, l);
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -60,12 +75,39 @@ __device__ __forceinline__ float act_value(uint32_t act, float z) {
         default:           return z;
     }
 }
+// of R x V values; one branch for all of them
+template <uint32_t ACT, int V, int R> __device__ __forceinline__ void act_each(float (&v)[R][V]) {
+#pragma unroll
+    for (int i = 0; i < R; i++)
+#pragma unroll
+        for (int j = 0; j < V; j++) v[i][j] = act_value(ACT, v[i][j]);
+}
+template <int V, int R> __device__ __forceinline__ void act_values(uint32_t act, float (&v)[R][V]) {
+    if (act == THC_ACT_NONE) return;
+    if (act == THC_ACT_RELU) act_each<THC_ACT_RELU>(v);
+    else if (act == THC_ACT_GELU) act_each<THC_ACT_GELU>(v);
+    else act_each<THC_ACT_SILU>(v);
+}
 __device__ __forceinline__ float act_slope(uint32_t act, float z) {
     switch (act) {
         case THC_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
         case THC_ACT_GELU: return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
         case THC_ACT_SILU: { const float s = 1.0f / (1.0f + expf(-z)); return s * (1.0f + z * (1.0f - s)); }
         default:           return 1.0f;
+    }
+}
+
+// v *= act'(z)
+template <int V> __device__ __forceinline__ void act_slopes(uint32_t act, float (&v)[V], const float (&z)[V]) {
+    if (act == THC_ACT_RELU) {
+#pragma unroll
+        for (int j = 0; j < V; j++) v[j] *= act_slope(THC_ACT_RELU, z[j]);
+    } else if (act == THC_ACT_GELU) {
+#pragma unroll
+        for (int j = 0; j < V; j++) v[j] *= act_slope(THC_ACT_GELU, z[j]);
+    } else if (act == THC_ACT_SILU) {
+#pragma unroll
+        for (int j = 0; j < V; j++) v[j] *= act_slope(THC_ACT_SILU, z[j]);
     }
 }
 

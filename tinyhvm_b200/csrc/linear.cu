@@ -49,37 +49,11 @@ __device__ __forceinline__ int scale_for(float top) {
     const int s = 14 - ((int)(__float_as_uint(top) >> 23) - 127);
     return s > 126 ? 126 : s;
 }
-template <int VEC> __device__ __forceinline__ void store_half(__half *p, const float (&v)[VEC]) {
-    if constexpr (VEC == 4) {
-        const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
-        *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
-    } else *p = __float2half_rn(v[0]);
-}
-template <int VEC> __device__ __forceinline__ void load4(const float *p, float (&v)[VEC]) {
-    if constexpr (VEC == 4) { const float4 q = *reinterpret_cast<const float4 *>(p); v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w; }
-    else v[0] = *p;
-}
-template <int VEC> __device__ __forceinline__ void load4(const __half *p, float (&v)[VEC]) {
-    if constexpr (VEC == 4) {
-        const uint2 q = *reinterpret_cast<const uint2 *>(p);
-        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&q.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&q.y));
-        v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
-    } else v[0] = __half2float(*p);
-}
-// hi and lo of v 2^s
-template <int VEC> __device__ __forceinline__ void put_planes(__half *hi, __half *lo, const float (&v)[VEC], float scale) {
-    float h[VEC], l[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; j++) { const float x = v[j] * scale; h[j] = __half2float(__float2half_rn(x)); l[j] = x - h[j]; }
-    store_half<VEC>(hi, h);
-    if (lo) store_half<VEC>(lo, l);
-}
-
 // what a row's values are
 template <typename T> struct RowsOf {                  // a matrix, its columns times 2^-shift
     const T *p; const int *shift; uint32_t cols;
     template <int VEC> __device__ void load(uint64_t row, uint32_t c, float (&v)[VEC]) const {
-        load4<VEC>(p + row * cols + c, v);
+        load_vec<VEC>(p + row * cols + c, v);
         if (shift) {
 #pragma unroll
             for (int j = 0; j < VEC; j++) v[j] *= pow2(-shift[c + j]);
@@ -89,12 +63,11 @@ template <typename T> struct RowsOf {                  // a matrix, its columns 
 template <typename T> struct GradOf {                  // dz = dy act'(z)
     const T *dy, *z; uint32_t cols, act;
     template <int VEC> __device__ void load(uint64_t row, uint32_t c, float (&v)[VEC]) const {
-        load4<VEC>(dy + row * cols + c, v);
+        load_vec<VEC>(dy + row * cols + c, v);
         if (act != THC_ACT_NONE) {
             float q[VEC];
-            load4<VEC>(z + row * cols + c, q);
-#pragma unroll
-            for (int j = 0; j < VEC; j++) v[j] *= act_slope(act, q[j]);
+            load_vec<VEC>(z + row * cols + c, q);
+            act_slopes<VEC>(act, v, q);
         }
     }
 };
@@ -144,7 +117,10 @@ k_split_rows(const Src src, const Planes out, uint32_t rows, uint32_t cols) {
 #pragma unroll
             for (int i = 0; i < U; i++) {
                 const uint32_t c = (threadIdx.x + 256u * i) * VEC;
-                if (c < cols) put_planes<VEC>(out.hi + row * out.pitch + c, out.lo ? out.lo + row * out.pitch + c : nullptr, v[i], scale);
+                if (c >= cols) continue;
+#pragma unroll
+                for (int j = 0; j < VEC; j++) v[i][j] *= scale;
+                store_planes<VEC>(out.hi + row * out.pitch + c, out.lo ? out.lo + row * out.pitch + c : nullptr, v[i]);
             }
         }
     }
@@ -174,7 +150,8 @@ k_split_long_rows(const Src src, const Planes out, uint32_t rows, uint32_t cols)
         }
         for (uint32_t c = threadIdx.x; c < cols; c += 256) {
             src.template load<1>(row, c, v);
-            put_planes<1>(out.hi + row * out.pitch + c, out.lo ? out.lo + row * out.pitch + c : nullptr, v, scale);
+            v[0] *= scale;
+            store_planes<1>(out.hi + row * out.pitch + c, out.lo ? out.lo + row * out.pitch + c : nullptr, v);
         }
     }
 }
@@ -214,7 +191,7 @@ k_col_tops(const T *x, const int *shift, float *tops, uint32_t rows, uint32_t co
     float top[VEC] = {};
     for (uint64_t row = blockIdx.y; row < rows; row += gridDim.y) {
         float v[VEC];
-        load4<VEC>(x + row * cols + c, v);
+        load_vec<VEC>(x + row * cols + c, v);
         const float f = pow2(-shift[row]);
 #pragma unroll
         for (int j = 0; j < VEC; j++) top[j] = fmaxf(top[j], finite_abs(v[j] * f));
@@ -238,11 +215,11 @@ k_split_cols(const T *x, const int *shift, const float *tops, const Planes out, 
     }
     for (uint64_t row = blockIdx.y; row < rows; row += gridDim.y) {
         float v[VEC];
-        load4<VEC>(x + row * cols + c, v);
+        load_vec<VEC>(x + row * cols + c, v);
         const float f = pow2(-shift[row]);
 #pragma unroll
         for (int j = 0; j < VEC; j++) v[j] = v[j] * f * scale[j];
-        put_planes<VEC>(out.hi + row * out.pitch + c, out.lo ? out.lo + row * out.pitch + c : nullptr, v, 1.0f);
+        store_planes<VEC>(out.hi + row * out.pitch + c, out.lo ? out.lo + row * out.pitch + c : nullptr, v);
     }
 }
 
@@ -278,37 +255,72 @@ struct Cut {
     uint8_t *base = nullptr;
     template <typename T> T *take(uint64_t n) { T *p = (T *)(base + at); at += (n * sizeof(T) + 255) & ~255ull; return p; }
 };
+// (rows of 64 values: the matrix engine may read them by blocks of 64 across)
 static Planes take_planes(Cut &c, uint32_t rows, uint32_t cols, bool lo, bool exps, uint32_t n_exps) {
     Planes p{};
-    p.pitch = (cols + 7u) & ~7ull;
-    p.hi = c.take<__half>(rows * p.pitch);
-    p.lo = lo ? c.take<__half>(rows * p.pitch) : nullptr;
+    p.pitch = (cols + 63u) & ~63ull;
+    p.hi = c.take<__half>(rows * p.pitch * (lo ? 2 : 1));
+    p.lo = lo ? p.hi + rows * p.pitch : nullptr;
     p.exps = exps ? c.take<int>(n_exps) : nullptr;
     return p;
 }
-static hg::Operand operand(const Planes &p, bool mn) { return hg::Operand{p.hi, p.lo, p.pitch, mn}; }
+static hg::Operand operand(const Planes &p, bool mn) { return hg::Operand{p.hi, p.pitch, p.lo ? (uint64_t)(p.lo - p.hi) : 0, mn}; }
 
 // ---- epilogue of a layer: out = act(sum 2^-exps + bias) + residual ----
 template <typename T> struct LayerEpi {
     static constexpr bool mirrors = false;
-    T *out, *z; const T *bias, *residual; const int *row_exps, *col_exps; uint32_t act, N;
-    float bias_n; int exp_n;                           // of the lane's column
-    __device__ void column(uint32_t n) { bias_n = bias ? to_f32(bias[n]) : 0.0f; exp_n = col_exps ? col_exps[n] : 0; }
-    __device__ void mirror(uint32_t, uint32_t, float) const {}
-    __device__ void put(uint32_t m, uint32_t n, float v, uint32_t) const {
-        const int e = -(row_exps ? row_exps[m] : 0) - exp_n, h = e >> 1;       // up to 252 either way: two exact factors
-        v = v * pow2(h) * pow2(e - h) + bias_n;
-        const uint64_t at = (uint64_t)m * N + n;
-        if (z) put_f32(z + at, v);
-        v = act_value(act, v);
-        if (residual) v += to_f32(residual[at]);
-        put_f32(out + at, v);
+    T *out, *z; const T *bias, *residual; const int *row_exps, *col_exps; uint32_t act, N;     // col_exps only beside row_exps
+    float bias_n[4]; int exp_n[4];                     // of the lane's columns
+    __device__ bool wide() const { return N % 4 == 0; }
+    template <int V> __device__ void column(uint32_t n) {
+#pragma unroll
+        for (int j = 0; j < V; j++) { if (bias) bias_n[j] = to_f32(bias[n + j]); if (col_exps) exp_n[j] = col_exps[n + j]; }
+    }
+    template <int V> __device__ void fetch(uint32_t m, uint32_t n, float (&x)[V]) const { if (residual) load_vec<V>(residual + (uint64_t)m * N + n, x); }
+    template <int V, int R> __device__ void put(hg::Rows r, uint32_t n, float (&v)[R][V], const float (&x)[R][V], uint32_t) const {
+        if (row_exps) {
+            int e[R];
+#pragma unroll
+            for (uint32_t i = 0; i < R; i++) { const uint32_t m = r.first + i * r.step; e[i] = m < r.end ? -row_exps[m] : 0; }
+            if (col_exps) {                            // up to 252 either way: two exact factors
+#pragma unroll
+                for (int i = 0; i < R; i++)
+#pragma unroll
+                    for (int j = 0; j < V; j++) { const int q = e[i] - exp_n[j], h = q >> 1; v[i][j] = v[i][j] * pow2(h) * pow2(q - h); }
+            } else {
+#pragma unroll
+                for (int i = 0; i < R; i++)
+#pragma unroll
+                    for (int j = 0; j < V; j++) v[i][j] *= pow2(e[i]);
+            }
+        }
+        if (bias) {
+#pragma unroll
+            for (int i = 0; i < R; i++)
+#pragma unroll
+                for (int j = 0; j < V; j++) v[i][j] += bias_n[j];
+        }
+        if (z) store<V, R>(z, r, n, v);
+        act_values<V, R>(act, v);
+        if (residual) {
+#pragma unroll
+            for (int i = 0; i < R; i++)
+#pragma unroll
+                for (int j = 0; j < V; j++) v[i][j] += x[i][j];
+        }
+        store<V, R>(out, r, n, v);
+    }
+    template <int V, int R> __device__ void store(T *to, hg::Rows r, uint32_t n, const float (&v)[R][V]) const {
+        T *p = to + (uint64_t)r.first * N + n;
+        const uint64_t step = (uint64_t)r.step * N;
+#pragma unroll
+        for (uint32_t i = 0; i < R; i++) if (r.first + i * r.step < r.end) store_vec<V>(p + i * step, v[i]);
     }
 };
 
 // an f16 matrix as it is, or copied to a pitch that tile loads can take
 static hg::Operand f16_operand(Cut &c, const __half *p, uint32_t rows, uint32_t cols, bool mn, bool copy) {
-    if (cols % 8 == 0) return hg::Operand{p, nullptr, cols, mn};
+    if (cols % 8 == 0) return hg::Operand{p, cols, 0, mn};
     const Planes q = take_planes(c, rows, cols, false, false, 0);
     if (copy) split_rows(RowsOf<__half>{p, nullptr, cols}, q, rows, cols, split_blocks(rows), "layer_operand");
     return operand(q, mn);
@@ -318,7 +330,7 @@ template <typename T>
 static void linear_forward(void *y, void *z, const void *x, const void *w, const void *bias, const void *residual, uint32_t M, uint32_t K, uint32_t N, uint32_t act) {
     constexpr bool F = sizeof(T) == 4;
     const hg::Plan plan = hg::plan(M, N, K, true);
-    LayerEpi<T> epi{(T *)y, (T *)z, (const T *)bias, (const T *)residual, nullptr, nullptr, act, N, 0.0f, 0};
+    LayerEpi<T> epi{(T *)y, (T *)z, (const T *)bias, (const T *)residual, nullptr, nullptr, act, N, {}, {}};
     Cut c;
     hg::Operand A{}, B{};
     float *partial = nullptr;
@@ -364,11 +376,11 @@ static void linear_backward(void *dx, void *dw, void *dbias, const void *dy, con
             k_fold_sums<T><<<(N + 31) / 32, 256, 0, g.stream>>>((T *)dbias, pz.sums, sum_rows, N);
             after_launch("linear_backward_bias");
         }
-        const hg::Operand dz_k = as_is ? hg::Operand{(const __half *)dy, nullptr, N, false} : operand(pz, false);
+        const hg::Operand dz_k = as_is ? hg::Operand{(const __half *)dy, N, 0, false} : operand(pz, false);
         hg::Operand dz_mn = dz_k;
         dz_mn.mn = true;
         if (dx) {
-            LayerEpi<T> epi{(T *)dx, nullptr, nullptr, nullptr, pz.exps, nullptr, THC_ACT_NONE, K, 0.0f, 0};
+            LayerEpi<T> epi{(T *)dx, nullptr, nullptr, nullptr, pz.exps, nullptr, THC_ACT_NONE, K, {}, {}};
             hg::Operand W{};
             if constexpr (F) {
                 const Planes pw = take_planes(c, K, N, true, true, K);
@@ -379,7 +391,7 @@ static void linear_backward(void *dx, void *dw, void *dbias, const void *dy, con
             if (pass) hg::product(dz_k, W, M, K, N, plan_x, partial, epi, false, "linear_backward_dx");
         }
         if (dw) {
-            LayerEpi<T> epi{(T *)dw, nullptr, nullptr, nullptr, nullptr, nullptr, THC_ACT_NONE, N, 0.0f, 0};
+            LayerEpi<T> epi{(T *)dw, nullptr, nullptr, nullptr, nullptr, nullptr, THC_ACT_NONE, N, {}, {}};
             hg::Operand X{};
             if (scaled) {                              // x takes dz's scales back
                 const Planes px = take_planes(c, M, K, F, true, K);

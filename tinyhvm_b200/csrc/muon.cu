@@ -18,12 +18,6 @@ constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 // 28262 and the low part's step is 2^-37.
 constexpr float PLANE = 8192.0f;
 
-__device__ __forceinline__ void put_plane(__half *hi, __half *lo, uint64_t at, float v) {
-    const __half h = __float2half_rn(v);
-    hi[at] = h;
-    lo[at] = __float2half_rn(v - __half2float(h));
-}
-
 // mom = mu mom + grad (when there is a momentum) and the sum of squares of the update: one partial per block, in double, which
 // the squares of f32 values do not overflow
 template <int VEC>
@@ -87,38 +81,78 @@ k_muon_planes(__half *hi, __half *lo, uint64_t pitch, const float *mom, const fl
             for (int j = 0; j < VEC; j++) u[j] = nesterov ? u[j] + mu * m[j] : m[j];
         }
 #pragma unroll
-        for (int j = 0; j < VEC; j++) put_plane(hi, lo, row * pitch + c + j, u[j] * f);
+        for (int j = 0; j < VEC; j++) u[j] *= f;
+        store_planes<VEC>(hi + row * pitch + c, lo + row * pitch + c, u);
     }
 }
 
 // ---- epilogues of the three products of a step (sums carry 2^26) ----
+template <int V, int R> __device__ __forceinline__ void times(float (&v)[R][V], float f) {
+#pragma unroll
+    for (int i = 0; i < R; i++)
+#pragma unroll
+        for (int j = 0; j < V; j++) v[i][j] *= f;
+}
+template <int V, int R> __device__ __forceinline__ void put_planes(__half *hi, __half *lo, uint64_t pitch, hg::Rows r, uint32_t n, const float (&v)[R][V]) {
+    const uint64_t at = r.first * pitch + n, step = r.step * pitch;
+#pragma unroll
+    for (uint32_t i = 0; i < R; i++) if (r.first + i * r.step < r.end) store_planes<V>(hi + at + i * step, lo + at + i * step, v[i]);
+}
 struct SquareEpi {                                     // A = X X^T
     static constexpr bool mirrors = true;
-    __half *hi, *lo; uint64_t pitch;
-    __device__ void column(uint32_t) const {}
-    __device__ void mirror(uint32_t n, uint32_t m, float v) const { put_plane(hi, lo, n * pitch + m, v * (1.0f / PLANE)); }
-    __device__ void put(uint32_t m, uint32_t n, float v, uint32_t) const { put_plane(hi, lo, m * pitch + n, v * (1.0f / PLANE)); }
+    __half *hi, *lo; uint64_t pitch; uint32_t side;
+    __device__ bool wide() const { return side % 4 == 0; }
+    template <int V> __device__ void column(uint32_t) const {}
+    template <int V> __device__ void fetch(uint32_t, uint32_t, float (&)[V]) const {}
+    template <int V, int R> __device__ void put(hg::Rows r, uint32_t n, float (&v)[R][V], const float (&)[R][V], uint32_t) const { mirror<V, R>(r, n, v); }
+    template <int V, int R> __device__ void mirror(hg::Rows r, uint32_t m, float (&v)[R][V]) const { times(v, 1.0f / PLANE); put_planes<V, R>(hi, lo, pitch, r, m, v); }
 };
 struct PolyEpi {                                       // a I + b A + c A A
     static constexpr bool mirrors = true;
-    __half *hi, *lo; const __half *a_hi, *a_lo; uint64_t pitch;
-    __device__ void column(uint32_t) const {}
-    __device__ float value(uint64_t at, float v) const { return NS_B * (__half2float(a_hi[at]) + __half2float(a_lo[at])) + NS_C * (v * (1.0f / PLANE)); }
-    __device__ void mirror(uint32_t n, uint32_t m, float v) const { const uint64_t at = n * pitch + m; put_plane(hi, lo, at, value(at, v)); }
-    __device__ void put(uint32_t m, uint32_t n, float v, uint32_t) const { const uint64_t at = m * pitch + n; put_plane(hi, lo, at, value(at, v) + (m == n ? NS_A * PLANE : 0.0f)); }
+    __half *hi, *lo; const __half *a_hi, *a_lo; uint64_t pitch; uint32_t side;
+    __device__ bool wide() const { return side % 4 == 0; }
+    template <int V> __device__ void column(uint32_t) const {}
+    template <int V> __device__ void fetch(uint32_t m, uint32_t n, float (&x)[V]) const {
+        float l[V];
+        load_vec<V>(a_hi + m * pitch + n, x);
+        load_vec<V>(a_lo + m * pitch + n, l);
+#pragma unroll
+        for (int j = 0; j < V; j++) x[j] += l[j];
+    }
+    template <int V, int R> __device__ void put(hg::Rows r, uint32_t n, float (&v)[R][V], const float (&x)[R][V], uint32_t) const {
+#pragma unroll
+        for (uint32_t i = 0; i < R; i++)
+#pragma unroll
+            for (int j = 0; j < V; j++) v[i][j] = NS_B * x[i][j] + NS_C * (v[i][j] * (1.0f / PLANE)) + (r.first + i * r.step == n + j ? NS_A * PLANE : 0.0f);
+        put_planes<V, R>(hi, lo, pitch, r, n, v);
+    }
+    template <int V, int R> __device__ void mirror(hg::Rows r, uint32_t m, float (&v)[R][V]) const {
+        float x[R][V];
+#pragma unroll
+        for (uint32_t i = 0; i < R; i++) if (r.first + i * r.step < r.end) fetch<V>(r.first + i * r.step, m, x[i]);
+        put<V, R>(r, m, v, x, 0);
+    }
 };
 struct ApplyEpi {                                      // X = (a I + b A + c A A) X: planes for the next step, the result, or the parameters' step
     static constexpr bool mirrors = false;
     __half *hi, *lo; uint64_t pitch;
     float *out, *param; uint32_t cols; float keep, step;
-    __device__ void column(uint32_t) const {}
-    __device__ void mirror(uint32_t, uint32_t, float) const {}
-    __device__ void put(uint32_t m, uint32_t n, float v, uint32_t) const {
-        if (hi) { put_plane(hi, lo, m * pitch + n, v * (1.0f / PLANE)); return; }
-        v *= 1.0f / (PLANE * PLANE);
-        const uint64_t at = (uint64_t)m * cols + n;
-        if (param) param[at] = param[at] * keep - step * v;
-        else out[at] = v;
+    __device__ bool wide() const { return cols % 4 == 0; }
+    template <int V> __device__ void column(uint32_t) const {}
+    template <int V> __device__ void fetch(uint32_t m, uint32_t n, float (&x)[V]) const { if (param) load_vec<V>(param + (uint64_t)m * cols + n, x); }
+    template <int V, int R> __device__ void put(hg::Rows r, uint32_t n, float (&v)[R][V], const float (&x)[R][V], uint32_t) const {
+        if (hi) { times(v, 1.0f / PLANE); put_planes<V, R>(hi, lo, pitch, r, n, v); return; }
+        times(v, 1.0f / (PLANE * PLANE));
+        if (param) {
+#pragma unroll
+            for (int i = 0; i < R; i++)
+#pragma unroll
+                for (int j = 0; j < V; j++) v[i][j] = x[i][j] * keep - step * v[i][j];
+        }
+        float *p = (param ? param : out) + (uint64_t)r.first * cols + n;
+        const uint64_t down = (uint64_t)r.step * cols;
+#pragma unroll
+        for (uint32_t i = 0; i < R; i++) if (r.first + i * r.step < r.end) store_vec<V>(p + i * down, v[i]);
     }
 };
 
@@ -127,7 +161,7 @@ static void newton_schulz(float *out, float *param, float *mom, const float *gra
     const uint64_t n = (uint64_t)rows * cols;
     const bool wide = rows <= cols;
     const uint32_t m = wide ? rows : cols, k = wide ? cols : rows;
-    const uint64_t px = (cols + 7u) & ~7ull, pm = (m + 7u) & ~7ull, x_bytes = (rows * px * 2 + 255) & ~255ull, m_bytes = (m * pm * 2 + 255) & ~255ull;
+    const uint64_t px = (cols + 63u) & ~63ull, pm = (m + 63u) & ~63ull, x_bytes = rows * px * 2, m_bytes = m * pm * 2;    // (multiples of 128)
     const unsigned blocks = grid_for(n, 1024, 4);
     const hg::Plan square = hg::plan(m, m, k, false), poly = hg::plan(m, m, m, false), apply = hg::plan(rows, cols, m, true);
     uint8_t *base = (uint8_t *)scratch_reserve(4 * x_bytes + 4 * m_bytes + apply.partial_bytes + blocks * sizeof(double));
@@ -149,12 +183,12 @@ static void newton_schulz(float *out, float *param, float *mom, const float *gra
     after_launch("newton_schulz_planes");
     for (uint32_t i = 0; i < steps; i++) {
         __half **cur = x[i & 1], **next = x[(i & 1) ^ 1];
-        const hg::Operand X{cur[0], cur[1], px, !wide}, A{a[0], a[1], pm, false}, B{b[0], b[1], pm, false};
-        hg::product(X, X, m, m, k, square, nullptr, SquareEpi{a[0], a[1], pm}, true, "newton_schulz_square");
-        hg::product(A, A, m, m, m, poly, nullptr, PolyEpi{b[0], b[1], a[0], a[1], pm}, true, "newton_schulz_poly");
+        const hg::Operand X{cur[0], px, rows * px, !wide}, A{a[0], pm, m * pm, false}, B{b[0], pm, m * pm, false};
+        hg::product(X, X, m, m, k, square, nullptr, SquareEpi{a[0], a[1], pm, m}, true, "newton_schulz_square");
+        hg::product(A, A, m, m, m, poly, nullptr, PolyEpi{b[0], b[1], a[0], a[1], pm, m}, true, "newton_schulz_poly");
         const bool last = i + 1 == steps;
-        const ApplyEpi epi{last ? nullptr : next[0], next[1], px, out, param, cols, keep, step};
-        const hg::Operand Xr{cur[0], cur[1], px, wide};                        // X across: the other way round than in its square
+        const ApplyEpi epi{last ? nullptr : next[0], next[1], px, out, last ? param : nullptr, cols, keep, step};
+        const hg::Operand Xr{cur[0], px, rows * px, wide};                        // X across: the other way round than in its square
         if (wide) hg::product(B, Xr, rows, cols, m, apply, partial, epi, false, "newton_schulz_apply");
         else hg::product(Xr, B, rows, cols, m, apply, partial, epi, false, "newton_schulz_apply");
     }
