@@ -9,7 +9,7 @@
 // product is below 2^-24): three f16 MMAs, where three tf32 MMAs would run at half their rate and keep 2^-21.
 //
 // The tensor core truncates when it adds to an accumulator, so a long sum drifts towards zero by about 2^-24 per add.
-// Here an accumulator lives for `chunk` blocks of 64 k only (2 with low planes, 8 without): eight epilogue warps then take it from
+// Here an accumulator lives for `chunk` blocks of 64 k only (2 with low planes, 16 without): eight epilogue warps then take it from
 // tensor memory and add it, rounded, to f32 sums in registers, while the MMAs of the next chunk fill the other of
 // two accumulators.  Within a block of k the small products go first.
 //
@@ -155,38 +155,53 @@ template <uint32_t NT> __device__ __forceinline__ Tile tile_of(const Shape &S, u
 
 // Epi: what happens to finished sums, R rows (m, m + step, ...; those below M count) of V neighbouring columns at a time (V = 4 where
 // Epi::wide() says that the result's rows allow it, else 1).  column<V>(n) sets up what belongs to the columns n, n+1, ...; fetch<V>(m, n, x)
-// reads what a row's result needs from memory; put<V, R>(rows, n, v, x, z) finishes and stores.  With Epi::mirrors, mirror<V, R> stores
+// reads what a row's result needs from memory; row_factor(m), exact, goes onto a row's sums before all that; put<V, R>(rows, n, v, x, z) finishes and stores.  With Epi::mirrors, mirror<V, R> stores
 // the transposed place of a symmetric product: rows along n, V neighbouring values of m.
-struct Rows { uint32_t first, step, end; };
+struct Rows { uint32_t first, step, end; };             // end: 0xffffffff where the caller knows that all are valid
 
 // A block of 32 x 32 sums passes through shared memory, one warp's 4 KB, from "a lane holds a row" to "eight lanes hold a row" (or
 // 32 lanes, V = 1).  16-byte chunk c of row r lies at chunk c ^ swap(r): whole rows, rows by chunk and columns by four are all read
 // and written without bank conflicts.
 //
-// Four rows of a lane go together, so that every choice the epilogue makes is one branch for all of them and their arithmetic
-// overlaps: two warps a scheduler hide no latency (row by row, a tile's epilogue took 18000 cycles; the MMAs of K = 1024 take 8000).
+// Four rows of a lane go together, so that their arithmetic overlaps.  What an epilogue does not do has to be left out when it is
+// compiled: a branch over sixteen values is turned into sixteen predicated instructions, and with every choice made at run time a
+// tile's epilogue took 18000 cycles, where the MMAs of K = 1024 take 8000 in f16.
 __device__ __forceinline__ uint32_t swap(uint32_t r) { return (r ^ (r >> 2)) & 7u; }
-template <int V, class Epi>
-__device__ __forceinline__ void put_block(Epi &e, const float *st, uint32_t lane, uint32_t m0, uint32_t n0, uint32_t M, uint32_t N, uint32_t z) {
-    constexpr uint32_t STEP = V == 4 ? 4 : 1;
-    const uint32_t ro = V == 4 ? lane >> 3 : 0u, n = n0 + (V == 4 ? (lane & 7u) * 4u : lane);
-    if (n >= N) return;
-    e.template column<V>(n);
-#pragma unroll 1
-    for (uint32_t r0 = ro; r0 < 32u; r0 += 4 * STEP) {
-        float x[4][V], v[4][V];
+template <int V, bool WHOLE, class Epi>
+__device__ __forceinline__ void put_block(Epi &e, const float *st, uint32_t lane, uint32_t m0, uint32_t n0, uint32_t rows, uint32_t N, uint32_t z) {
+    const uint32_t M = WHOLE ? 0xffffffffu : rows;
+    if constexpr (V == 4) {
+        const uint32_t ro = lane >> 3, n = n0 + (lane & 7u) * 4u, b = (lane & 7u) ^ ro;
+        if (!WHOLE && n >= N) return;
+        e.template column<4>(n);
+        const float *p = st + ro * 32u;
 #pragma unroll
-        for (uint32_t i = 0; i < 4; i++)
-            if (m0 + r0 + i * STEP < M) e.template fetch<V>(m0 + r0 + i * STEP, n, x[i]);
+        for (uint32_t t = 0; t < 8; t += 4) {          // row ro + 4 t: swap(ro + 4 t) = ro ^ (4 (t & 1)) ^ t
+            float x[4][4], v[4][4];
 #pragma unroll
-        for (uint32_t i = 0; i < 4; i++) {
-            const uint32_t r = r0 + i * STEP;
-            if constexpr (V == 4) {
-                const float4 q = *reinterpret_cast<const float4 *>(st + r * 32u + (((lane & 7u) ^ swap(r)) << 2));
+            for (uint32_t i = 0; i < 4; i++)
+                if (m0 + ro + 4 * (t + i) < M) e.template fetch<4>(m0 + ro + 4 * (t + i), n, x[i]);
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+                const float4 q = *reinterpret_cast<const float4 *>(p + (t + i) * 128u + ((b ^ (((i & 1u) * 4u) ^ (t + i))) << 2));
                 v[i][0] = q.x; v[i][1] = q.y; v[i][2] = q.z; v[i][3] = q.w;
-            } else v[i][0] = st[r * 32u + (((lane >> 2) ^ swap(r)) << 2) + (lane & 3u)];
+            }
+            e.template put<4, 4>(Rows{m0 + ro + 4 * t, 4, M}, n, v, x, z);
         }
-        e.template put<V, 4>(Rows{m0 + r0, STEP, M}, n, v, x, z);
+    } else {
+        const uint32_t n = n0 + lane;
+        if (n >= N) return;
+        e.template column<1>(n);
+#pragma unroll 1
+        for (uint32_t r0 = 0; r0 < 32u; r0 += 4) {
+            float x[4][1], v[4][1];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+                if (m0 + r0 + i < M) e.template fetch<1>(m0 + r0 + i, n, x[i]);
+                v[i][0] = st[(r0 + i) * 32u + (((lane >> 2) ^ swap(r0 + i)) << 2) + (lane & 3u)];
+            }
+            e.template put<1, 4>(Rows{m0 + r0, 1, M}, n, v, x, z);
+        }
     }
 }
 template <int V, class Epi>
@@ -285,6 +300,7 @@ k_hgemm(const __grid_constant__ Shape S, const __grid_constant__ Maps maps, cons
             }
             if (!ok) break;
             const uint32_t m0 = T.m0 + rank * 128u + q * 32u, n0 = T.n0 + half * COLS;
+            const float f = m0 + lane < S.M ? e.row_factor(m0 + lane) : 0.0f;
 #pragma unroll 1
             for (uint32_t j = 0; j < COLS / 32; j++) {
                 const uint32_t n1 = n0 + j * 32u;
@@ -295,7 +311,7 @@ k_hgemm(const __grid_constant__ Shape S, const __grid_constant__ Maps maps, cons
                     if (k == j) {
 #pragma unroll
                         for (uint32_t i = 0; i < 8; i++)
-                            *reinterpret_cast<float4 *>(st + lane * 32u + ((i ^ swap(lane)) << 2)) = make_float4(acc[k * 32 + 4 * i], acc[k * 32 + 4 * i + 1], acc[k * 32 + 4 * i + 2], acc[k * 32 + 4 * i + 3]);
+                            *reinterpret_cast<float4 *>(st + lane * 32u + ((i ^ swap(lane)) << 2)) = make_float4(acc[k * 32 + 4 * i] * f, acc[k * 32 + 4 * i + 1] * f, acc[k * 32 + 4 * i + 2] * f, acc[k * 32 + 4 * i + 3] * f);
                     }
                 __syncwarp();
                 bool above = false;
@@ -306,8 +322,9 @@ k_hgemm(const __grid_constant__ Shape S, const __grid_constant__ Maps maps, cons
                         above = true;
                     }
                 }
-                if (wide) put_block<4>(e, st, lane, m0, n1, S.M, S.N, T.z);
-                else put_block<1>(e, st, lane, m0, n1, S.M, S.N, T.z);
+                if (wide && m0 + 32u <= S.M && n1 + 32u <= S.N) put_block<4, true>(e, st, lane, m0, n1, S.M, S.N, T.z);
+                else if (wide) put_block<4, false>(e, st, lane, m0, n1, S.M, S.N, T.z);
+                else put_block<1, false>(e, st, lane, m0, n1, S.M, S.N, T.z);
                 if constexpr (Epi::mirrors) {
                     if (above) { if (wide) mirror_block<4>(e, st, lane, m0, n1, S.N); else mirror_block<1>(e, st, lane, m0, n1, S.N); }
                 }
@@ -399,6 +416,7 @@ struct PartialEpi {
     static constexpr bool mirrors = false;
     float *partial; uint64_t mn; uint32_t N;
     __device__ bool wide() const { return N % 4 == 0; }
+    __device__ float row_factor(uint32_t) const { return 1.0f; }
     template <int V> __device__ void column(uint32_t) const {}
     template <int V> __device__ void fetch(uint32_t, uint32_t, float (&)[V]) const {}
     template <int V, int R> __device__ void put(Rows r, uint32_t n, const float (&v)[R][V], const float (&)[R][V], uint32_t z) const {
@@ -423,6 +441,9 @@ k_hgemm_fold(const float *partial, uint32_t splits, uint32_t M, uint32_t N, cons
 #pragma unroll
             for (int j = 0; j < V; j++) v[0][j] += p[j];
         }
+        const float f = e.row_factor(m);
+#pragma unroll
+        for (int j = 0; j < V; j++) v[0][j] *= f;
         e.template put<V, 1>(Rows{m, 1, M}, n, v, x, 0);
     }
 }
@@ -505,7 +526,7 @@ static void product(const Operand &A, const Operand &B, uint32_t M, uint32_t N, 
     S.split_blocks = (S.blocks + p.splits - 1) / p.splits;
     S.splits = p.splits;
     S.a_lo = A.plane != 0; S.b_lo = B.plane != 0;
-    S.chunk = S.a_lo || S.b_lo ? 2 : 8;
+    S.chunk = S.a_lo || S.b_lo ? 2 : 16;
     S.a_bytes = A_PLANE * (1 + S.a_lo);
     S.stage_bytes = S.a_bytes + p.nt / 2 * 128 * (1 + S.b_lo);
     S.stages = RING_BYTES / S.stage_bytes;

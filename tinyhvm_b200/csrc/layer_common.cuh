@@ -75,19 +75,6 @@ __device__ __forceinline__ float act_value(uint32_t act, float z) {
         default:           return z;
     }
 }
-// of R x V values; one branch for all of them
-template <uint32_t ACT, int V, int R> __device__ __forceinline__ void act_each(float (&v)[R][V]) {
-#pragma unroll
-    for (int i = 0; i < R; i++)
-#pragma unroll
-        for (int j = 0; j < V; j++) v[i][j] = act_value(ACT, v[i][j]);
-}
-template <int V, int R> __device__ __forceinline__ void act_values(uint32_t act, float (&v)[R][V]) {
-    if (act == THC_ACT_NONE) return;
-    if (act == THC_ACT_RELU) act_each<THC_ACT_RELU>(v);
-    else if (act == THC_ACT_GELU) act_each<THC_ACT_GELU>(v);
-    else act_each<THC_ACT_SILU>(v);
-}
 __device__ __forceinline__ float act_slope(uint32_t act, float z) {
     switch (act) {
         case THC_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;

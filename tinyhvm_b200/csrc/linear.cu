@@ -266,55 +266,58 @@ static Planes take_planes(Cut &c, uint32_t rows, uint32_t cols, bool lo, bool ex
 }
 static hg::Operand operand(const Planes &p, bool mn) { return hg::Operand{p.hi, p.pitch, p.lo ? (uint64_t)(p.lo - p.hi) : 0, mn}; }
 
-// ---- epilogue of a layer: out = act(sum 2^-exps + bias) + residual ----
-template <typename T> struct LayerEpi {
+// ---- epilogues: what a layer stores, and a gradient ----
+template <typename T, int V, int R> __device__ __forceinline__ void store_rows(T *to, hg::Rows r, uint32_t n, uint32_t N, const float (&v)[R][V]) {
+    T *p = to + (uint64_t)r.first * N + n;
+    const uint64_t step = (uint64_t)r.step * N;
+#pragma unroll
+    for (uint32_t i = 0; i < R; i++, p += step) if (r.first + i * r.step < r.end) store_vec<V>(p, v[i]);
+}
+template <typename T, uint32_t ACT> struct LayerEpi {  // act(sum 2^-exps[m] + bias) + residual
     static constexpr bool mirrors = false;
-    T *out, *z; const T *bias, *residual; const int *row_exps, *col_exps; uint32_t act, N;     // col_exps only beside row_exps
-    float bias_n[4]; int exp_n[4];                     // of the lane's columns
+    T *out, *z; const T *bias, *residual; const int *exps; uint32_t N;
+    float bias_n[4];                                   // of the lane's columns
     __device__ bool wide() const { return N % 4 == 0; }
+    __device__ float row_factor(uint32_t m) const { return exps ? pow2(-exps[m]) : 1.0f; }
     template <int V> __device__ void column(uint32_t n) {
 #pragma unroll
-        for (int j = 0; j < V; j++) { if (bias) bias_n[j] = to_f32(bias[n + j]); if (col_exps) exp_n[j] = col_exps[n + j]; }
+        for (int j = 0; j < V; j++) bias_n[j] = bias ? to_f32(bias[n + j]) : 0.0f;
     }
     template <int V> __device__ void fetch(uint32_t m, uint32_t n, float (&x)[V]) const { if (residual) load_vec<V>(residual + (uint64_t)m * N + n, x); }
     template <int V, int R> __device__ void put(hg::Rows r, uint32_t n, float (&v)[R][V], const float (&x)[R][V], uint32_t) const {
-        if (row_exps) {
-            int e[R];
 #pragma unroll
-            for (uint32_t i = 0; i < R; i++) { const uint32_t m = r.first + i * r.step; e[i] = m < r.end ? -row_exps[m] : 0; }
-            if (col_exps) {                            // up to 252 either way: two exact factors
+        for (int i = 0; i < R; i++)
 #pragma unroll
-                for (int i = 0; i < R; i++)
+            for (int j = 0; j < V; j++) v[i][j] += bias_n[j];
+        if (z) store_rows<T, V, R>(z, r, n, N, v);
 #pragma unroll
-                    for (int j = 0; j < V; j++) { const int q = e[i] - exp_n[j], h = q >> 1; v[i][j] = v[i][j] * pow2(h) * pow2(q - h); }
-            } else {
+        for (int i = 0; i < R; i++)
 #pragma unroll
-                for (int i = 0; i < R; i++)
-#pragma unroll
-                    for (int j = 0; j < V; j++) v[i][j] *= pow2(e[i]);
-            }
-        }
-        if (bias) {
-#pragma unroll
-            for (int i = 0; i < R; i++)
-#pragma unroll
-                for (int j = 0; j < V; j++) v[i][j] += bias_n[j];
-        }
-        if (z) store<V, R>(z, r, n, v);
-        act_values<V, R>(act, v);
-        if (residual) {
-#pragma unroll
-            for (int i = 0; i < R; i++)
-#pragma unroll
-                for (int j = 0; j < V; j++) v[i][j] += x[i][j];
-        }
-        store<V, R>(out, r, n, v);
+            for (int j = 0; j < V; j++) { v[i][j] = act_value(ACT, v[i][j]); if (residual) v[i][j] += x[i][j]; }
+        store_rows<T, V, R>(out, r, n, N, v);
     }
-    template <int V, int R> __device__ void store(T *to, hg::Rows r, uint32_t n, const float (&v)[R][V]) const {
-        T *p = to + (uint64_t)r.first * N + n;
-        const uint64_t step = (uint64_t)r.step * N;
+};
+template <typename T, bool COLS> struct GradEpi {      // sum 2^(-exps[m] - col_exps[n])
+    static constexpr bool mirrors = false;
+    T *out; const int *exps, *col_exps; uint32_t N;
+    int exp_n[4];
+    __device__ bool wide() const { return N % 4 == 0; }
+    __device__ float row_factor(uint32_t m) const { return !COLS && exps ? pow2(-exps[m]) : 1.0f; }
+    template <int V> __device__ void column(uint32_t n) {
+        if constexpr (COLS) {
 #pragma unroll
-        for (uint32_t i = 0; i < R; i++) if (r.first + i * r.step < r.end) store_vec<V>(p + i * step, v[i]);
+            for (int j = 0; j < V; j++) exp_n[j] = col_exps[n + j];
+        }
+    }
+    template <int V> __device__ void fetch(uint32_t m, uint32_t, float (&x)[V]) const { if constexpr (COLS) x[0] = __int_as_float(exps[m]); }
+    template <int V, int R> __device__ void put(hg::Rows r, uint32_t n, float (&v)[R][V], const float (&x)[R][V], uint32_t) const {
+        if constexpr (COLS) {                          // up to 252 either way: two exact factors
+#pragma unroll
+            for (int i = 0; i < R; i++)
+#pragma unroll
+                for (int j = 0; j < V; j++) { const int e = -__float_as_int(x[i][0]) - exp_n[j], h = e >> 1; v[i][j] = v[i][j] * pow2(h) * pow2(e - h); }
+        }
+        store_rows<T, V, R>(out, r, n, N, v);
     }
 };
 
@@ -330,7 +333,7 @@ template <typename T>
 static void linear_forward(void *y, void *z, const void *x, const void *w, const void *bias, const void *residual, uint32_t M, uint32_t K, uint32_t N, uint32_t act) {
     constexpr bool F = sizeof(T) == 4;
     const hg::Plan plan = hg::plan(M, N, K, true);
-    LayerEpi<T> epi{(T *)y, (T *)z, (const T *)bias, (const T *)residual, nullptr, nullptr, act, N, {}, {}};
+    const int *exps = nullptr;
     Cut c;
     hg::Operand A{}, B{};
     float *partial = nullptr;
@@ -340,7 +343,7 @@ static void linear_forward(void *y, void *z, const void *x, const void *w, const
         if constexpr (F) {
             const Planes pw = take_planes(c, K, N, true, true, K), px = take_planes(c, M, K, true, true, M);
             A = operand(px, false); B = operand(pw, true);
-            epi.row_exps = px.exps;
+            exps = px.exps;
             if (pass) {
                 split_rows(RowsOf<float>{(const float *)w, nullptr, N}, pw, K, N, split_blocks(K), "layer_operand");
                 split_rows(RowsOf<float>{(const float *)x, pw.exps, K}, px, M, K, split_blocks(M), "layer_operand");
@@ -350,7 +353,15 @@ static void linear_forward(void *y, void *z, const void *x, const void *w, const
             B = f16_operand(c, (const __half *)w, K, N, true, pass);
         }
     }
-    hg::product(A, B, M, N, K, plan, partial, epi, false, "linear");
+    const auto run = [&](auto epi) { hg::product(A, B, M, N, K, plan, partial, epi, false, "linear"); };
+    T *ty = (T *)y, *tz = (T *)z;
+    const T *tb = (const T *)bias, *tr = (const T *)residual;
+    switch (act) {
+        case THC_ACT_RELU: run(LayerEpi<T, THC_ACT_RELU>{ty, tz, tb, tr, exps, N, {}}); break;
+        case THC_ACT_GELU: run(LayerEpi<T, THC_ACT_GELU>{ty, tz, tb, tr, exps, N, {}}); break;
+        case THC_ACT_SILU: run(LayerEpi<T, THC_ACT_SILU>{ty, tz, tb, tr, exps, N, {}}); break;
+        default:           run(LayerEpi<T, THC_ACT_NONE>{ty, tz, tb, tr, exps, N, {}}); break;
+    }
 }
 
 template <typename T>
@@ -380,19 +391,19 @@ static void linear_backward(void *dx, void *dw, void *dbias, const void *dy, con
         hg::Operand dz_mn = dz_k;
         dz_mn.mn = true;
         if (dx) {
-            LayerEpi<T> epi{(T *)dx, nullptr, nullptr, nullptr, pz.exps, nullptr, THC_ACT_NONE, K, {}, {}};
             hg::Operand W{};
+            const int *col_exps = nullptr;
             if constexpr (F) {
                 const Planes pw = take_planes(c, K, N, true, true, K);
                 if (pass) split_rows(RowsOf<float>{(const float *)w, nullptr, N}, pw, K, N, split_blocks(K), "layer_operand");
                 W = operand(pw, false);
-                epi.col_exps = pw.exps;
+                col_exps = pw.exps;
             } else W = f16_operand(c, (const __half *)w, K, N, false, pass);
-            if (pass) hg::product(dz_k, W, M, K, N, plan_x, partial, epi, false, "linear_backward_dx");
+            if (pass) hg::product(dz_k, W, M, K, N, plan_x, partial, GradEpi<T, F>{(T *)dx, pz.exps, col_exps, K, {}}, false, "linear_backward_dx");
         }
         if (dw) {
-            LayerEpi<T> epi{(T *)dw, nullptr, nullptr, nullptr, nullptr, nullptr, THC_ACT_NONE, N, {}, {}};
             hg::Operand X{};
+            const int *exps = nullptr;
             if (scaled) {                              // x takes dz's scales back
                 const Planes px = take_planes(c, M, K, F, true, K);
                 float *tops = c.take<float>((uint64_t)runs * K);
@@ -409,9 +420,9 @@ static void linear_backward(void *dx, void *dw, void *dbias, const void *dy, con
                     after_launch("layer_operand");
                 }
                 X = operand(px, true);
-                epi.row_exps = px.exps;
+                exps = px.exps;
             } else if constexpr (!F) X = f16_operand(c, (const __half *)x, M, K, true, pass);
-            if (pass) hg::product(X, dz_mn, K, N, M, plan_w, partial, epi, false, "linear_backward_dw");
+            if (pass) hg::product(X, dz_mn, K, N, M, plan_w, partial, GradEpi<T, false>{(T *)dw, exps, nullptr, N, {}}, false, "linear_backward_dw");
         }
     }
 }

@@ -87,12 +87,6 @@ k_muon_planes(__half *hi, __half *lo, uint64_t pitch, const float *mom, const fl
 }
 
 // ---- epilogues of the three products of a step (sums carry 2^26) ----
-template <int V, int R> __device__ __forceinline__ void times(float (&v)[R][V], float f) {
-#pragma unroll
-    for (int i = 0; i < R; i++)
-#pragma unroll
-        for (int j = 0; j < V; j++) v[i][j] *= f;
-}
 template <int V, int R> __device__ __forceinline__ void put_planes(__half *hi, __half *lo, uint64_t pitch, hg::Rows r, uint32_t n, const float (&v)[R][V]) {
     const uint64_t at = r.first * pitch + n, step = r.step * pitch;
 #pragma unroll
@@ -102,15 +96,17 @@ struct SquareEpi {                                     // A = X X^T
     static constexpr bool mirrors = true;
     __half *hi, *lo; uint64_t pitch; uint32_t side;
     __device__ bool wide() const { return side % 4 == 0; }
+    __device__ float row_factor(uint32_t) const { return 1.0f / PLANE; }
     template <int V> __device__ void column(uint32_t) const {}
     template <int V> __device__ void fetch(uint32_t, uint32_t, float (&)[V]) const {}
     template <int V, int R> __device__ void put(hg::Rows r, uint32_t n, float (&v)[R][V], const float (&)[R][V], uint32_t) const { mirror<V, R>(r, n, v); }
-    template <int V, int R> __device__ void mirror(hg::Rows r, uint32_t m, float (&v)[R][V]) const { times(v, 1.0f / PLANE); put_planes<V, R>(hi, lo, pitch, r, m, v); }
+    template <int V, int R> __device__ void mirror(hg::Rows r, uint32_t m, float (&v)[R][V]) const { put_planes<V, R>(hi, lo, pitch, r, m, v); }
 };
 struct PolyEpi {                                       // a I + b A + c A A
     static constexpr bool mirrors = true;
     __half *hi, *lo; const __half *a_hi, *a_lo; uint64_t pitch; uint32_t side;
     __device__ bool wide() const { return side % 4 == 0; }
+    __device__ float row_factor(uint32_t) const { return 1.0f / PLANE; }
     template <int V> __device__ void column(uint32_t) const {}
     template <int V> __device__ void fetch(uint32_t m, uint32_t n, float (&x)[V]) const {
         float l[V];
@@ -123,7 +119,7 @@ struct PolyEpi {                                       // a I + b A + c A A
 #pragma unroll
         for (uint32_t i = 0; i < R; i++)
 #pragma unroll
-            for (int j = 0; j < V; j++) v[i][j] = NS_B * x[i][j] + NS_C * (v[i][j] * (1.0f / PLANE)) + (r.first + i * r.step == n + j ? NS_A * PLANE : 0.0f);
+            for (int j = 0; j < V; j++) v[i][j] = NS_B * x[i][j] + NS_C * v[i][j] + (r.first + i * r.step == n + j ? NS_A * PLANE : 0.0f);
         put_planes<V, R>(hi, lo, pitch, r, n, v);
     }
     template <int V, int R> __device__ void mirror(hg::Rows r, uint32_t m, float (&v)[R][V]) const {
@@ -133,26 +129,27 @@ struct PolyEpi {                                       // a I + b A + c A A
         put<V, R>(r, m, v, x, 0);
     }
 };
-struct ApplyEpi {                                      // X = (a I + b A + c A A) X: planes for the next step, the result, or the parameters' step
+enum { NEXT, RESULT, STEP };
+template <int TO> struct ApplyEpi {                    // X = (a I + b A + c A A) X: planes for the next step, the result, or the parameters' step
     static constexpr bool mirrors = false;
     __half *hi, *lo; uint64_t pitch;
-    float *out, *param; uint32_t cols; float keep, step;
+    float *out; uint32_t cols; float keep, step;
     __device__ bool wide() const { return cols % 4 == 0; }
+    __device__ float row_factor(uint32_t) const { return TO == NEXT ? 1.0f / PLANE : 1.0f / (PLANE * PLANE); }
     template <int V> __device__ void column(uint32_t) const {}
-    template <int V> __device__ void fetch(uint32_t m, uint32_t n, float (&x)[V]) const { if (param) load_vec<V>(param + (uint64_t)m * cols + n, x); }
+    template <int V> __device__ void fetch(uint32_t m, uint32_t n, float (&x)[V]) const { if constexpr (TO == STEP) load_vec<V>(out + (uint64_t)m * cols + n, x); }
     template <int V, int R> __device__ void put(hg::Rows r, uint32_t n, float (&v)[R][V], const float (&x)[R][V], uint32_t) const {
-        if (hi) { times(v, 1.0f / PLANE); put_planes<V, R>(hi, lo, pitch, r, n, v); return; }
-        times(v, 1.0f / (PLANE * PLANE));
-        if (param) {
-#pragma unroll
-            for (int i = 0; i < R; i++)
-#pragma unroll
-                for (int j = 0; j < V; j++) v[i][j] = x[i][j] * keep - step * v[i][j];
-        }
-        float *p = (param ? param : out) + (uint64_t)r.first * cols + n;
+        if constexpr (TO == NEXT) { put_planes<V, R>(hi, lo, pitch, r, n, v); return; }
+        float *p = out + (uint64_t)r.first * cols + n;
         const uint64_t down = (uint64_t)r.step * cols;
 #pragma unroll
-        for (uint32_t i = 0; i < R; i++) if (r.first + i * r.step < r.end) store_vec<V>(p + i * down, v[i]);
+        for (uint32_t i = 0; i < R; i++, p += down) {
+            if constexpr (TO == STEP) {
+#pragma unroll
+                for (int j = 0; j < V; j++) v[i][j] = x[i][j] * keep - step * v[i][j];
+            }
+            if (r.first + i * r.step < r.end) store_vec<V>(p, v[i]);
+        }
     }
 };
 
@@ -186,11 +183,11 @@ static void newton_schulz(float *out, float *param, float *mom, const float *gra
         const hg::Operand X{cur[0], px, rows * px, !wide}, A{a[0], pm, m * pm, false}, B{b[0], pm, m * pm, false};
         hg::product(X, X, m, m, k, square, nullptr, SquareEpi{a[0], a[1], pm, m}, true, "newton_schulz_square");
         hg::product(A, A, m, m, m, poly, nullptr, PolyEpi{b[0], b[1], a[0], a[1], pm, m}, true, "newton_schulz_poly");
-        const bool last = i + 1 == steps;
-        const ApplyEpi epi{last ? nullptr : next[0], next[1], px, out, last ? param : nullptr, cols, keep, step};
-        const hg::Operand Xr{cur[0], px, rows * px, wide};                        // X across: the other way round than in its square
-        if (wide) hg::product(B, Xr, rows, cols, m, apply, partial, epi, false, "newton_schulz_apply");
-        else hg::product(Xr, B, rows, cols, m, apply, partial, epi, false, "newton_schulz_apply");
+        const hg::Operand Xr{cur[0], px, rows * px, wide};                     // X across: the other way round than in its square
+        const auto run = [&](auto epi) { hg::product(wide ? B : Xr, wide ? Xr : B, rows, cols, m, apply, partial, epi, false, "newton_schulz_apply"); };
+        if (i + 1 < steps) run(ApplyEpi<NEXT>{next[0], next[1], px, nullptr, cols, 0.0f, 0.0f});
+        else if (param) run(ApplyEpi<STEP>{nullptr, nullptr, 0, param, cols, keep, step});
+        else run(ApplyEpi<RESULT>{nullptr, nullptr, 0, out, cols, 0.0f, 0.0f});
     }
 }
 
