@@ -127,6 +127,11 @@ __device__ __forceinline__ void acc_load(uint32_t addr, uint32_t (&r)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// `n` values of a row into L2
+template <typename T> __device__ __forceinline__ void touch_row(const T *row, uint32_t from, uint32_t n, uint32_t end) {
+    for (uint32_t i = from; i < from + n && i < end; i += 128u / sizeof(T)) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + i));
+}
+
 struct Tile { uint32_t m0, n0, z, blocks, block0; };
 // Tiles in order: split, then bands of 8 row tiles, columns, rows of the band: the tiles in flight share few operand panels.
 template <uint32_t NT> __device__ __forceinline__ Tile tile_of(const Shape &S, uint32_t t) {
@@ -278,6 +283,8 @@ k_hgemm(const __grid_constant__ Shape S, const __grid_constant__ Maps maps, cons
         uint32_t c = 0;                                    // chunks so far
         for (uint32_t t = pair; t < S.tiles && ok; t += pairs) {
             const Tile T = tile_of<NT>(S, t);
+            const uint32_t m0 = T.m0 + rank * 128u + q * 32u, n0 = T.n0 + half * COLS;
+            if (m0 + lane < S.M) e.touch(m0 + lane, n0, COLS);         // what the result reads: into L2 while the sums are made
             float acc[COLS];
 #pragma unroll
             for (uint32_t i = 0; i < COLS; i++) acc[i] = 0.0f;
@@ -299,7 +306,6 @@ k_hgemm(const __grid_constant__ Shape S, const __grid_constant__ Maps maps, cons
                 if (lane == 0) bar_arrive(in_cta(smem32(&sh.acc_empty[buf]), 0));
             }
             if (!ok) break;
-            const uint32_t m0 = T.m0 + rank * 128u + q * 32u, n0 = T.n0 + half * COLS;
             const float f = m0 + lane < S.M ? e.row_factor(m0 + lane) : 0.0f;
 #pragma unroll 1
             for (uint32_t j = 0; j < COLS / 32; j++) {
@@ -417,6 +423,7 @@ struct PartialEpi {
     float *partial; uint64_t mn; uint32_t N;
     __device__ bool wide() const { return N % 4 == 0; }
     __device__ float row_factor(uint32_t) const { return 1.0f; }
+    __device__ void touch(uint32_t, uint32_t, uint32_t) const {}
     template <int V> __device__ void column(uint32_t) const {}
     template <int V> __device__ void fetch(uint32_t, uint32_t, float (&)[V]) const {}
     template <int V, int R> __device__ void put(Rows r, uint32_t n, const float (&v)[R][V], const float (&)[R][V], uint32_t z) const {

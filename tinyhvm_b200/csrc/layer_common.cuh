@@ -67,23 +67,39 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 
 // ---- activations (thvm_cuda_linear): value and slope at z ----
+// Phi(z) = (1 + erf(z / sqrt 2)) / 2.  With t = |z| / sqrt 2, erfc(t) = 2^(-t p(t)); p is a polynomial of degree 7 fitted to
+// -log2(erfc(t)) / t over [0, 4] so that erf's error is least at its largest (1.6e-8, with f32 arithmetic 7.5e-8; beyond 4, where
+// erfc < 2e-8, t p(t) keeps growing).  One exponential and no branch, where erff has two; the lower tail keeps its relative accuracy.
+__device__ __forceinline__ float normal_cdf(float z) {
+    const float t = fabsf(z) * 0.70710678f;
+    float p = 4.5354569e-05f;
+    p = fmaf(p, t, -4.4547446e-04f);
+    p = fmaf(p, t, 1.4893346e-03f);
+    p = fmaf(p, t, 7.7480281e-04f);
+    p = fmaf(p, t, -2.8253829e-02f);
+    p = fmaf(p, t, 1.4848168e-01f);
+    p = fmaf(p, t, 9.1841638e-01f);
+    p = fmaf(p, t, 1.6279086f);
+    const float half_erfc = 0.5f * exp2f(-t * p);
+    return z < 0.0f ? half_erfc : 1.0f - half_erfc;
+}
+__device__ __forceinline__ float logistic(float z) { return __fdividef(1.0f, 1.0f + exp2f(-1.44269504f * z)); }
 __device__ __forceinline__ float act_value(uint32_t act, float z) {
     switch (act) {
         case THC_ACT_RELU: return z > 0.0f ? z : 0.0f;                       // as the RELU op of the dispatch path: NaN gives 0
-        case THC_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-        case THC_ACT_SILU: return z / (1.0f + expf(-z));                     // z = -inf: -inf / inf is NaN, as the formula says
+        case THC_ACT_GELU: return z * normal_cdf(z);
+        case THC_ACT_SILU: return z * logistic(z);
         default:           return z;
     }
 }
 __device__ __forceinline__ float act_slope(uint32_t act, float z) {
     switch (act) {
         case THC_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
-        case THC_ACT_GELU: return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
-        case THC_ACT_SILU: { const float s = 1.0f / (1.0f + expf(-z)); return s * (1.0f + z * (1.0f - s)); }
+        case THC_ACT_GELU: return normal_cdf(z) + z * exp2f(-0.72134752f * z * z) * 0.39894228f;
+        case THC_ACT_SILU: { const float s = logistic(z); return s * (1.0f + z * (1.0f - s)); }
         default:           return 1.0f;
     }
 }
-
 // v *= act'(z)
 template <int V> __device__ __forceinline__ void act_slopes(uint32_t act, float (&v)[V], const float (&z)[V]) {
     if (act == THC_ACT_RELU) {

@@ -279,6 +279,7 @@ template <typename T, uint32_t ACT> struct LayerEpi {  // act(sum 2^-exps[m] + b
     float bias_n[4];                                   // of the lane's columns
     __device__ bool wide() const { return N % 4 == 0; }
     __device__ float row_factor(uint32_t m) const { return exps ? pow2(-exps[m]) : 1.0f; }
+    __device__ void touch(uint32_t m, uint32_t n, uint32_t cols) const { if (residual) hg::touch_row(residual + (uint64_t)m * N, n, cols, N); }
     template <int V> __device__ void column(uint32_t n) {
 #pragma unroll
         for (int j = 0; j < V; j++) bias_n[j] = bias ? to_f32(bias[n + j]) : 0.0f;
@@ -303,6 +304,7 @@ template <typename T, bool COLS> struct GradEpi {      // sum 2^(-exps[m] - col_
     int exp_n[4];
     __device__ bool wide() const { return N % 4 == 0; }
     __device__ float row_factor(uint32_t m) const { return !COLS && exps ? pow2(-exps[m]) : 1.0f; }
+    __device__ void touch(uint32_t, uint32_t, uint32_t) const {}
     template <int V> __device__ void column(uint32_t n) {
         if constexpr (COLS) {
 #pragma unroll

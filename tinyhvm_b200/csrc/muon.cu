@@ -97,6 +97,7 @@ struct SquareEpi {                                     // A = X X^T
     __half *hi, *lo; uint64_t pitch; uint32_t side;
     __device__ bool wide() const { return side % 4 == 0; }
     __device__ float row_factor(uint32_t) const { return 1.0f / PLANE; }
+    __device__ void touch(uint32_t, uint32_t, uint32_t) const {}
     template <int V> __device__ void column(uint32_t) const {}
     template <int V> __device__ void fetch(uint32_t, uint32_t, float (&)[V]) const {}
     template <int V, int R> __device__ void put(hg::Rows r, uint32_t n, float (&v)[R][V], const float (&)[R][V], uint32_t) const { mirror<V, R>(r, n, v); }
@@ -107,6 +108,7 @@ struct PolyEpi {                                       // a I + b A + c A A
     __half *hi, *lo; const __half *a_hi, *a_lo; uint64_t pitch; uint32_t side;
     __device__ bool wide() const { return side % 4 == 0; }
     __device__ float row_factor(uint32_t) const { return 1.0f / PLANE; }
+    __device__ void touch(uint32_t, uint32_t, uint32_t) const {}
     template <int V> __device__ void column(uint32_t) const {}
     template <int V> __device__ void fetch(uint32_t m, uint32_t n, float (&x)[V]) const {
         float l[V];
@@ -135,6 +137,7 @@ template <int TO> struct ApplyEpi {                    // X = (a I + b A + c A A
     __half *hi, *lo; uint64_t pitch;
     float *out; uint32_t cols; float keep, step;
     __device__ bool wide() const { return cols % 4 == 0; }
+    __device__ void touch(uint32_t m, uint32_t n, uint32_t count) const { if constexpr (TO == STEP) hg::touch_row(out + (uint64_t)m * cols, n, count, cols); }
     __device__ float row_factor(uint32_t) const { return TO == NEXT ? 1.0f / PLANE : 1.0f / (PLANE * PLANE); }
     template <int V> __device__ void column(uint32_t) const {}
     template <int V> __device__ void fetch(uint32_t m, uint32_t n, float (&x)[V]) const { if constexpr (TO == STEP) load_vec<V>(out + (uint64_t)m * cols + n, x); }
