@@ -9,7 +9,7 @@
 // product is below 2^-24): three f16 MMAs, where three tf32 MMAs would run at half their rate and keep 2^-21.
 //
 // The tensor core truncates when it adds to an accumulator, so a long sum drifts towards zero by about 2^-24 per add.
-// Here an accumulator lives for `chunk` blocks of 64 k only (2 with low planes, 16 without): eight epilogue warps then take it from
+// Here an accumulator lives for 128 k only (1024 without low planes): eight epilogue warps then take it from
 // tensor memory and add it, rounded, to f32 sums in registers, while the MMAs of the next chunk fill the other of
 // two accumulators.  Within a block of k the small products go first.
 //
@@ -34,8 +34,8 @@ namespace thc {
 namespace hg {
 
 constexpr uint32_t EPI_WARPS = 8, TMA_A_WARP = 8, TMA_B_WARP = 9, MMA_WARP = 10, THREADS = 384;
-// 168 registers a thread at launch (65536 / 384, by eights); the epilogue's two warpgroups take from the third: 128 x 40 + 256 x 232 = 384 x 168
-constexpr uint32_t EPI_REGS = 232, IO_REGS = 40;
+// 168 registers a thread at launch (65536 / 384, by eights); the epilogue's two warpgroups take from the third: 128 x 56 + 256 x 224 = 384 x 168
+constexpr uint32_t EPI_REGS = 224, IO_REGS = 56;
 constexpr uint32_t KB = 64;                                // k of a block: 128 bytes, the swizzle's width
 constexpr uint32_t A_PLANE = 128 * 128;                    // bytes of one CTA's A plane of a block
 constexpr uint32_t RING_BYTES = 196608, STAGING = EPI_WARPS * 4096;
@@ -57,9 +57,9 @@ constexpr size_t SMEM = 1024 + RING_BYTES + STAGING + sizeof(Shared);
 struct Shape {
     uint32_t M, N, K;
     uint32_t row_tiles, col_tiles, tiles;                  // tiles: of all splits, below the diagonal left out when `upper`
-    uint32_t blocks, split_blocks, chunk;                  // blocks of 64 k: in all, per split, per chunk
+    uint32_t blocks, split_blocks, chunk;                  // blocks of k: in all, per split, per chunk
     uint32_t splits;
-    uint32_t stages, stage_bytes, a_bytes;
+    uint32_t halves, stages, stage_bytes, half_bytes, a_bytes;   // a block of k is one or two times 64 k: a half holds A's and B's planes of 64 k
     uint32_t a_mode, b_mode, a_lo, b_lo, upper;
     int *status;
 };
@@ -84,6 +84,19 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
                      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
         if (ok) return true;
         if ((it & 255u) == 255u && *abort_flag) return false;
+    }
+    *abort_flag = 1;
+    return false;
+}
+// The same for the three threads that everything waits for: test_wait in a tight loop, as try_wait may park the thread and waking it
+// takes several hundred cycles.
+__device__ __forceinline__ bool bar_spin(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
+    for (uint32_t it = 0; it < WAIT_LIMIT * 8u; ++it) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
+        if ((it & 1023u) == 1023u && *abort_flag) return false;
     }
     *abort_flag = 1;
     return false;
@@ -341,17 +354,18 @@ k_hgemm(const __grid_constant__ Shape S, const __grid_constant__ Maps maps, cons
         if (lane == 0) {
             const bool is_a = warp == TMA_A_WARP;
             const CUtensorMap *map = is_a ? &maps.a : &maps.b;
-            const uint32_t mode = is_a ? S.a_mode : S.b_mode, boxes = is_a ? 2u : NT / 128, width = is_a ? 128u : NT / 2, at = is_a ? 0u : S.a_bytes;
+            const uint32_t halves = S.halves, mode = is_a ? S.a_mode : S.b_mode, boxes = is_a ? 2u : NT / 128, width = is_a ? 128u : NT / 2, at = is_a ? 0u : S.a_bytes;
             bool ok = true;
             uint32_t it = 0, s = 0, use = 0;
             for (uint32_t t = pair; t < S.tiles && ok; t += pairs) {
                 const Tile T = tile_of<NT>(S, t);
                 const uint32_t mn = (is_a ? T.m0 : T.n0) + rank * width;
                 for (uint32_t kb = 0; kb < T.blocks; kb++) {
-                    if (use) ok = bar_wait(smem32(&sh.empty[s]), (use - 1) & 1u, abort_flag);
+                    if (use) ok = bar_spin(smem32(&sh.empty[s]), (use - 1) & 1u, abort_flag);
                     if (!ok) break;
                     if (is_a && rank == 0) bar_expect(smem32(&sh.full[s]), 2u * S.stage_bytes);
-                    load_operand(ring + s * S.stage_bytes + at, map, in_cta(smem32(&sh.full[s]), 0), mode, boxes, mn, (T.block0 + kb) * KB);
+                    const uint32_t dst = ring + s * S.stage_bytes + at, bar = in_cta(smem32(&sh.full[s]), 0), k = (T.block0 + kb) * halves;
+                    for (uint32_t h = 0; h < halves; h++) load_operand(dst + h * S.half_bytes, map, bar, mode, boxes, mn, (k + h) * KB);
                     it++;
                     if (++s == S.stages) { s = 0; use++; }
                 }
@@ -370,35 +384,38 @@ k_hgemm(const __grid_constant__ Shape S, const __grid_constant__ Maps maps, cons
             const uint32_t a_mn = S.a_mode != K_ROWS, b_mn = S.b_mode != K_ROWS;
             const uint32_t idesc = (1u << 4) | (a_mn << 15) | (b_mn << 16) | ((NT >> 3) << 17) | ((256u >> 4) << 24);   // f32 sums of f16 products
             const uint64_t step_a = a_mn ? 2048u >> 4 : 32u >> 4, step_b = b_mn ? 2048u >> 4 : 32u >> 4;                 // 16 k further
+            const uint32_t lo = S.a_lo | S.b_lo << 1, halves = S.halves, chunk = S.chunk, stages = S.stages;
+            const uint64_t a_first = operand_desc(ring, a_mn), b_first = operand_desc(ring + S.a_bytes, b_mn), half = S.half_bytes >> 4;
             bool ok = true;
             uint32_t s = 0, use = 0, c = 0;
+            uint64_t at = 0;                               // of the stage, in the descriptors' units
             for (uint32_t t = pair; t < S.tiles && ok; t += pairs) {
                 const Tile T = tile_of<NT>(S, t);
-                for (uint32_t kb = 0; kb < T.blocks && ok; kb += S.chunk, c++) {
+                for (uint32_t kb = 0; kb < T.blocks && ok; kb += chunk, c++) {
                     const uint32_t buf = c & 1u, d = tmem + buf * NT;
-                    if (c >= 2) ok = bar_wait(smem32(&sh.acc_empty[buf]), ((c >> 1) - 1) & 1u, abort_flag);
-                    const uint32_t end = T.blocks - kb < S.chunk ? T.blocks - kb : S.chunk;
+                    if (c >= 2) ok = bar_spin(smem32(&sh.acc_empty[buf]), ((c >> 1) - 1) & 1u, abort_flag);
+                    const uint32_t end = T.blocks - kb < chunk ? T.blocks - kb : chunk;
                     uint32_t more = 0;
                     for (uint32_t i = 0; i < end && ok; i++) {
-                        ok = bar_wait(smem32(&sh.full[s]), use & 1u, abort_flag);
+                        ok = bar_spin(smem32(&sh.full[s]), use & 1u, abort_flag);
                         if (!ok) break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        const uint32_t sa = ring + s * S.stage_bytes, sb = sa + S.a_bytes;
-                        const uint64_t a_hi = operand_desc(sa, a_mn), b_hi = operand_desc(sb, b_mn);
-                        if (S.a_lo) {
-                            const uint64_t a_lo = operand_desc(sa + A_PLANE, a_mn);
+                        uint64_t a_hi = a_first + at, b_hi = b_first + at;
+                        for (uint32_t h = 0; h < halves; h++, a_hi += half, b_hi += half) {
+                            if (lo & 1u) {
 #pragma unroll
-                            for (uint32_t k = 0; k < 4; k++) { mma(d, a_lo + k * step_a, b_hi + k * step_b, idesc, more); more = 1; }
+                                for (uint32_t k = 0; k < 4; k++) { mma(d, a_hi + (A_PLANE >> 4) + k * step_a, b_hi + k * step_b, idesc, more); more = 1; }
+                            }
+                            if (lo & 2u) {
+#pragma unroll
+                                for (uint32_t k = 0; k < 4; k++) { mma(d, a_hi + k * step_a, b_hi + (B_PLANE >> 4) + k * step_b, idesc, more); more = 1; }
+                            }
+#pragma unroll
+                            for (uint32_t k = 0; k < 4; k++) { mma(d, a_hi + k * step_a, b_hi + k * step_b, idesc, more); more = 1; }
                         }
-                        if (S.b_lo) {
-                            const uint64_t b_lo = operand_desc(sb + B_PLANE, b_mn);
-#pragma unroll
-                            for (uint32_t k = 0; k < 4; k++) { mma(d, a_hi + k * step_a, b_lo + k * step_b, idesc, more); more = 1; }
-                        }
-#pragma unroll
-                        for (uint32_t k = 0; k < 4; k++) { mma(d, a_hi + k * step_a, b_hi + k * step_b, idesc, more); more = 1; }
                         commit_both(smem32(&sh.empty[s]));
-                        if (++s == S.stages) { s = 0; use++; }
+                        at += S.stage_bytes >> 4;
+                        if (++s == stages) { s = 0; use++; at = 0; }
                     }
                     if (ok) commit_both(smem32(&sh.acc_full[buf]));
                 }
@@ -529,29 +546,31 @@ static void product(const Operand &A, const Operand &B, uint32_t M, uint32_t N, 
     memset(&S, 0, sizeof S);
     S.M = M; S.N = N; S.K = K;
     S.row_tiles = (M + 255) / 256; S.col_tiles = (N + p.nt - 1) / p.nt;
-    S.blocks = (K + KB - 1) / KB;
+    S.halves = A.plane || B.plane ? 1 : 2;
+    S.blocks = (K + KB * S.halves - 1) / (KB * S.halves);
     S.split_blocks = (S.blocks + p.splits - 1) / p.splits;
-    S.splits = p.splits;
+    S.splits = (S.blocks + S.split_blocks - 1) / S.split_blocks;        // (p.splits or fewer)
     S.a_lo = A.plane != 0; S.b_lo = B.plane != 0;
-    S.chunk = S.a_lo || S.b_lo ? 2 : 16;
+    S.chunk = S.a_lo || S.b_lo ? 2 : 8;
     S.a_bytes = A_PLANE * (1 + S.a_lo);
-    S.stage_bytes = S.a_bytes + p.nt / 2 * 128 * (1 + S.b_lo);
+    S.half_bytes = S.a_bytes + p.nt / 2 * 128 * (1 + S.b_lo);
+    S.stage_bytes = S.half_bytes * S.halves;
     S.stages = RING_BYTES / S.stage_bytes;
     if (S.stages > MAX_STAGES) S.stages = MAX_STAGES;
     S.upper = upper;
-    S.tiles = S.row_tiles * S.col_tiles * p.splits;
+    S.tiles = S.row_tiles * S.col_tiles * S.splits;
     if (upper) { S.tiles = 0; for (uint32_t r = 0; r < S.row_tiles; r++) S.tiles += S.col_tiles - r * 256 / p.nt; }
     S.status = g.dev_status;
     Maps maps;
     S.a_mode = operand_map(&maps.a, A, M, K, 128);
     S.b_mode = operand_map(&maps.b, B, N, K, p.nt / 2);
-    if constexpr (!Epi::mirrors) if (p.splits > 1) {
+    if constexpr (!Epi::mirrors) if (S.splits > 1) {
         const PartialEpi pe{partial, (uint64_t)M * N, N};
         if (p.nt == 256) launch<256>(S, maps, pe, name); else launch<128>(S, maps, pe, name);
         profile_begin();
         const uint32_t down = (M + 7) / 8 < 4096 ? (M + 7) / 8 : 4096;
-        if (N % 4 == 0) k_hgemm_fold<4, Epi><<<dim3((N + 127) / 128, down), 256, 0, g.stream>>>(partial, p.splits, M, N, epi);
-        else k_hgemm_fold<1, Epi><<<dim3((N + 31) / 32, down), 256, 0, g.stream>>>(partial, p.splits, M, N, epi);
+        if (N % 4 == 0) k_hgemm_fold<4, Epi><<<dim3((N + 127) / 128, down), 256, 0, g.stream>>>(partial, S.splits, M, N, epi);
+        else k_hgemm_fold<1, Epi><<<dim3((N + 31) / 32, down), 256, 0, g.stream>>>(partial, S.splits, M, N, epi);
         after_launch("layer_fold");
         return;
     }
