@@ -28,6 +28,7 @@
 #include <string.h>
 #include <unordered_map>
 #include "layer_common.cuh"
+#include "layer_host.h"
 #include "state.h"
 
 namespace thc {
@@ -58,7 +59,7 @@ struct Shape {
     uint32_t M, N, K;
     uint32_t row_tiles, col_tiles, tiles;                  // tiles: of all splits, below the diagonal left out when `upper`
     uint32_t blocks, split_blocks, chunk;                  // blocks of k: in all, per split, per chunk
-    uint32_t splits;
+    uint32_t split_tiles;                                  // tiles of a split
     uint32_t halves, stages, stage_bytes, half_bytes, a_bytes;   // a block of k is one or two times 64 k: a half holds A's and B's planes of 64 k
     uint32_t a_mode, b_mode, a_lo, b_lo, upper;
     int *status;
@@ -150,6 +151,8 @@ struct Tile { uint32_t m0, n0, z, blocks, block0; };
 template <uint32_t NT> __device__ __forceinline__ Tile tile_of(const Shape &S, uint32_t t) {
     Tile r;
     uint32_t row, col;
+    r.z = t / S.split_tiles;
+    t -= r.z * S.split_tiles;
     if (S.upper) {                                         // row by row from the diagonal on
         row = 0; col = t;
         for (;;) {
@@ -157,11 +160,8 @@ template <uint32_t NT> __device__ __forceinline__ Tile tile_of(const Shape &S, u
             if (col < n) { col += first; break; }
             col -= n; row++;
         }
-        r.z = 0;
     } else {
-        const uint32_t per = S.row_tiles * S.col_tiles;
-        r.z = t / per;
-        const uint32_t u = t - r.z * per, band = u / (8u * S.col_tiles), v = u - band * 8u * S.col_tiles;
+        const uint32_t band = t / (8u * S.col_tiles), v = t - band * 8u * S.col_tiles;
         const uint32_t h = S.row_tiles - band * 8u < 8u ? S.row_tiles - band * 8u : 8u;
         col = v / h; row = band * 8u + (v - col * h);
     }
@@ -238,23 +238,6 @@ __device__ __forceinline__ void mirror_block(Epi &e, const float *st, uint32_t l
         e.template mirror<V, 4>(Rows{n0 + c0, STEP, N}, m0 + mo, v);
     }
 }
-// a block on the diagonal: each value decides for itself
-template <class Epi>
-__device__ __forceinline__ void diagonal_block(Epi &e, const float *st, uint32_t lane, uint32_t m0, uint32_t n0, uint32_t M, uint32_t N) {
-    const uint32_t n = n0 + lane;
-    if (n >= N) return;
-#pragma unroll 1
-    for (uint32_t r = 0; r < 32u; r++) {
-        const uint32_t m = m0 + r;
-        if (m > n || m >= M) break;
-        const float s = st[r * 32u + (((lane >> 2) ^ swap(r)) << 2) + (lane & 3u)];
-        float x[1][1], v[1][1] = {{s}}, w[1][1] = {{s}};
-        e.template fetch<1>(m, n, x[0]);
-        e.template put<1, 1>(Rows{m, 1, M}, n, v, x, 0);
-        if (m < n) e.template mirror<1, 1>(Rows{n, 1, N}, m, w);
-    }
-}
-
 template <uint32_t NT, class Epi>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 k_hgemm(const __grid_constant__ Shape S, const __grid_constant__ Maps maps, const __grid_constant__ Epi epi) {
@@ -279,6 +262,7 @@ k_hgemm(const __grid_constant__ Shape S, const __grid_constant__ Maps maps, cons
     __syncthreads();
     cluster_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    depend();
     const uint32_t tmem = sh.tmem;
     const uint32_t ring = smem32(base);
     constexpr uint32_t B_PLANE = NT / 2 * 128;             // bytes of this CTA's B plane of a block
@@ -336,9 +320,8 @@ k_hgemm(const __grid_constant__ Shape S, const __grid_constant__ Maps maps, cons
                 bool above = false;
                 if constexpr (Epi::mirrors) {
                     if (S.upper) {
-                        if (n1 + 31u < m0) continue;
-                        if (n1 <= m0 + 31u) { diagonal_block(e, st, lane, m0, n1, S.M, S.N); continue; }
-                        above = true;
+                        if (n1 < m0) continue;                 // (blocks of 32 x 32: below the diagonal the mirror of one above writes)
+                        above = n1 > m0;
                     }
                 }
                 if (wide && m0 + 32u <= S.M && n1 + 32u <= S.N) put_block<4, true>(e, st, lane, m0, n1, S.M, S.N, T.z);
@@ -453,6 +436,7 @@ __global__ void __launch_bounds__(256)
 k_hgemm_fold(const float *partial, uint32_t splits, uint32_t M, uint32_t N, const __grid_constant__ Epi epi) {
     const uint32_t n = (blockIdx.x * 32 + (threadIdx.x & 31u)) * V;
     if (n >= N) return;
+    depend();
     Epi e = epi;
     e.template column<V>(n);
     for (uint32_t m = blockIdx.y * 8 + (threadIdx.x >> 5); m < M; m += gridDim.y * 8) {
@@ -469,6 +453,46 @@ k_hgemm_fold(const float *partial, uint32_t splits, uint32_t M, uint32_t N, cons
 #pragma unroll
         for (int j = 0; j < V; j++) v[0][j] *= f;
         e.template put<V, 1>(Rows{m, 1, M}, n, v, x, 0);
+    }
+}
+
+// The same for a symmetric product, of which only the tiles from the diagonal on were made: a block of 256 threads takes 32 x 32 sums
+// on or above it and writes them in both places.  Through shared memory as in the product's own epilogue, one warp's layout.
+template <int V, class Epi>
+__global__ void __launch_bounds__(256)
+k_hgemm_fold_upper(const float *partial, uint32_t splits, uint32_t M, const __grid_constant__ Epi epi) {
+    if (blockIdx.x < blockIdx.y) return;
+    depend();
+    __shared__ float st[32][33];
+    const uint32_t m0 = blockIdx.y * 32, n0 = blockIdx.x * 32, lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    Epi e = epi;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; i++) {
+        const uint32_t m = m0 + warp + 8 * i, n = n0 + lane;
+        float v = 0.0f;
+        if (m < M && n < M) {
+            for (uint32_t z = 0; z < splits; z++) v += partial[((uint64_t)z * M + m) * M + n];
+            v *= e.row_factor(m);
+        }
+        st[warp + 8 * i][lane] = v;
+    }
+    __syncthreads();
+    constexpr uint32_t PER = 32 / V;                       // threads a row
+    for (uint32_t u = threadIdx.x; u < 32 * PER; u += 256) {
+        const uint32_t r = u / PER, c = (u % PER) * V;
+        float x[1][V], v[1][V];
+        if (m0 + r < M && n0 + c < M) {
+#pragma unroll
+            for (uint32_t j = 0; j < V; j++) v[0][j] = st[r][c + j];
+            e.template column<V>(n0 + c);
+            e.template fetch<V>(m0 + r, n0 + c, x[0]);
+            e.template put<V, 1>(Rows{m0 + r, 1, M}, n0 + c, v, x, 0);
+        }
+        if (blockIdx.x > blockIdx.y && n0 + r < M && m0 + c < M) {
+#pragma unroll
+            for (uint32_t j = 0; j < V; j++) v[0][j] = st[c + j][r];
+            e.template mirror<V, 1>(Rows{n0 + r, 1, M}, m0 + c, v);
+        }
     }
 }
 
@@ -511,19 +535,22 @@ static uint32_t operand_map(CUtensorMap *m, const Operand &o, uint32_t rows, uin
 }
 
 struct Plan { uint32_t nt, splits; uint64_t partial_bytes; };
+static uint32_t count_tiles(uint32_t M, uint32_t N, uint32_t nt, bool upper) {
+    const uint32_t rows = (M + 255) / 256, cols = (N + nt - 1) / nt;
+    uint32_t n = rows * cols;
+    if (upper) { n = 0; for (uint32_t r = 0; r < rows; r++) n += cols - r * 256 / nt; }
+    return n;
+}
 // Tile width and splits for an M x N product over K.  Wide tiles halve the traffic of A's panels, but a grid that leaves
-// pairs idle loses more: narrow ones then, and below half a grid K is split as well, into runs of at least 4 blocks of 64.
-static Plan plan(uint32_t M, uint32_t N, uint32_t K, bool may_split) {
-    const uint32_t pairs = (uint32_t)g.sm_count / 2, rows = (M + 255) / 256;
+// pairs idle loses more: narrow ones then, and below half a grid K is split as well, into runs of at least 512 (the sums of a split
+// go through memory and a second kernel, some 5 us, which is what the products of 1024 k take).
+static Plan plan(uint32_t M, uint32_t N, uint32_t K, bool upper) {
+    const uint32_t pairs = (uint32_t)g.sm_count / 2;
     Plan p;
-    p.nt = (uint64_t)rows * ((N + 255) / 256) >= pairs ? 256 : 128;
-    const uint64_t tiles = (uint64_t)rows * ((N + p.nt - 1) / p.nt);
-    const uint32_t blocks = (K + KB - 1) / KB;
-    uint64_t s = may_split ? pairs / tiles : 1;
-    if (s > blocks / 4) s = blocks / 4;
-    if (s < 1) s = 1;
-    const uint32_t per = (uint32_t)((blocks + s - 1) / s);
-    p.splits = (blocks + per - 1) / per;
+    p.nt = count_tiles(M, N, 256, upper) >= pairs ? 256 : 128;
+    const uint32_t tiles = count_tiles(M, N, p.nt, upper), most = K / 512;
+    p.splits = pairs / tiles < most ? pairs / tiles : most;
+    if (p.splits < 1) p.splits = 1;
     p.partial_bytes = p.splits > 1 ? (uint64_t)p.splits * M * N * 4 : 0;
     return p;
 }
@@ -534,7 +561,7 @@ static void launch(const Shape &S, const Maps &maps, const Epi &epi, const char 
     if (!ready) { THC_CUDA_OK(cudaFuncSetAttribute(k_hgemm<NT, Epi>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM)); ready = true; }
     const uint32_t pairs = (uint32_t)g.sm_count / 2;
     profile_begin();
-    k_hgemm<NT, Epi><<<2 * (S.tiles < pairs ? S.tiles : pairs), THREADS, SMEM, g.stream>>>(S, maps, epi);
+    chain(k_hgemm<NT, Epi>, dim3(2 * (S.tiles < pairs ? S.tiles : pairs)), THREADS, SMEM, S, maps, epi);
     after_launch(name);
 }
 
@@ -549,7 +576,7 @@ static void product(const Operand &A, const Operand &B, uint32_t M, uint32_t N, 
     S.halves = A.plane || B.plane ? 1 : 2;
     S.blocks = (K + KB * S.halves - 1) / (KB * S.halves);
     S.split_blocks = (S.blocks + p.splits - 1) / p.splits;
-    S.splits = (S.blocks + S.split_blocks - 1) / S.split_blocks;        // (p.splits or fewer)
+    const uint32_t splits = (S.blocks + S.split_blocks - 1) / S.split_blocks;          // p.splits or fewer
     S.a_lo = A.plane != 0; S.b_lo = B.plane != 0;
     S.chunk = S.a_lo || S.b_lo ? 2 : 8;
     S.a_bytes = A_PLANE * (1 + S.a_lo);
@@ -558,19 +585,25 @@ static void product(const Operand &A, const Operand &B, uint32_t M, uint32_t N, 
     S.stages = RING_BYTES / S.stage_bytes;
     if (S.stages > MAX_STAGES) S.stages = MAX_STAGES;
     S.upper = upper;
-    S.tiles = S.row_tiles * S.col_tiles * S.splits;
-    if (upper) { S.tiles = 0; for (uint32_t r = 0; r < S.row_tiles; r++) S.tiles += S.col_tiles - r * 256 / p.nt; }
+    S.split_tiles = count_tiles(M, N, p.nt, upper);
+    S.tiles = S.split_tiles * splits;
     S.status = g.dev_status;
     Maps maps;
     S.a_mode = operand_map(&maps.a, A, M, K, 128);
     S.b_mode = operand_map(&maps.b, B, N, K, p.nt / 2);
-    if constexpr (!Epi::mirrors) if (S.splits > 1) {
+    if (splits > 1) {
         const PartialEpi pe{partial, (uint64_t)M * N, N};
         if (p.nt == 256) launch<256>(S, maps, pe, name); else launch<128>(S, maps, pe, name);
         profile_begin();
-        const uint32_t down = (M + 7) / 8 < 4096 ? (M + 7) / 8 : 4096;
-        if (N % 4 == 0) k_hgemm_fold<4, Epi><<<dim3((N + 127) / 128, down), 256, 0, g.stream>>>(partial, S.splits, M, N, epi);
-        else k_hgemm_fold<1, Epi><<<dim3((N + 31) / 32, down), 256, 0, g.stream>>>(partial, S.splits, M, N, epi);
+        if constexpr (Epi::mirrors) {
+            const dim3 grid((N + 31) / 32, (M + 31) / 32);
+            if (N % 4 == 0) chain(k_hgemm_fold_upper<4, Epi>, grid, 256, 0, (const float *)partial, splits, M, epi);
+            else chain(k_hgemm_fold_upper<1, Epi>, grid, 256, 0, (const float *)partial, splits, M, epi);
+        } else {
+            const uint32_t down = (M + 7) / 8 < 4096 ? (M + 7) / 8 : 4096;
+            if (N % 4 == 0) chain(k_hgemm_fold<4, Epi>, dim3((N + 127) / 128, down), 256, 0, (const float *)partial, splits, M, N, epi);
+            else chain(k_hgemm_fold<1, Epi>, dim3((N + 31) / 32, down), 256, 0, (const float *)partial, splits, M, N, epi);
+        }
         after_launch("layer_fold");
         return;
     }

@@ -11,6 +11,13 @@
 
 namespace thc {
 
+// Kernels of these operators follow one another as dependent launches (layer_host.h:chain): a kernel may be set up while the one before
+// it still runs.  Each calls this before it touches memory: everything before is then finished and visible, and the kernel after may be set up.
+__device__ __forceinline__ void depend() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ void put_f32(float *p, float v) { *p = v; }

@@ -52,6 +52,7 @@ constexpr int NORM_VALUES = 32;                        // values of a row that a
 template <typename T, int VEC, int G>
 __global__ void __launch_bounds__(G > 32 ? G : NORM_BLOCK)
 k_norm(T *y, float *mean_out, float *rstd_out, const T *x, const T *gamma, const T *beta, uint32_t rows, uint32_t cols, float eps) {
+    depend();
     constexpr int NV = NORM_VALUES / VEC;
     __shared__ float red[G > 32 ? G / 32 : 1];
     const uint32_t t = G > 32 ? threadIdx.x : (threadIdx.x & 31u);
@@ -109,6 +110,7 @@ k_norm(T *y, float *mean_out, float *rstd_out, const T *x, const T *gamma, const
 template <typename T>
 __global__ void __launch_bounds__(1024)
 k_norm_long(T *y, float *mean_out, float *rstd_out, const T *x, const T *gamma, const T *beta, uint32_t rows, uint32_t cols, float eps) {
+    depend();
     __shared__ float red[32];
     for (uint64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const T *xr = x + row * cols;
@@ -137,6 +139,7 @@ constexpr int NORM_BWD_VALUES = 8;                     // values of a row that a
 template <typename T, int VEC, int G>
 __global__ void __launch_bounds__(G > 32 ? G : NORM_BLOCK)
 k_norm_bwd(T *dx, float *partial, const T *dy, const T *x, const T *gamma, const float *mean, const float *rstd, uint32_t rows, uint32_t cols) {
+    depend();
     constexpr int NV = NORM_BWD_VALUES / VEC, R = G > 32 ? 1 : NORM_BLOCK / 32;
     __shared__ float2 red[G > 32 ? G / 32 : 1];
     __shared__ float fold[G > 32 ? 1 : NORM_BLOCK * NORM_BWD_VALUES];
@@ -221,6 +224,7 @@ k_norm_bwd(T *dx, float *partial, const T *dy, const T *x, const T *gamma, const
 template <typename T>
 __global__ void __launch_bounds__(1024)
 k_norm_bwd_long(T *dx, const T *dy, const T *x, const T *gamma, const float *mean, const float *rstd, uint32_t rows, uint32_t cols) {
+    depend();
     __shared__ float2 red[32];
     for (uint64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const float mu = mean[row], rs = rstd[row];
@@ -241,6 +245,7 @@ k_norm_bwd_long(T *dx, const T *dy, const T *x, const T *gamma, const float *mea
 template <typename T>
 __global__ void __launch_bounds__(256)
 k_norm_bwd_cols(float *partial, const T *dy, const T *x, const float *mean, const float *rstd, uint32_t rows, uint32_t cols) {
+    depend();
     const uint32_t c = blockIdx.x * 256 + threadIdx.x;
     if (c >= cols) return;
     float sg = 0.0f, sb = 0.0f;
@@ -256,6 +261,7 @@ k_norm_bwd_cols(float *partial, const T *dy, const T *x, const float *mean, cons
 template <typename T>
 __global__ void __launch_bounds__(256)
 k_norm_fold(T *dgamma, T *dbeta, const float *partial, uint32_t n, uint32_t cols) {
+    depend();
     __shared__ float red[8][33];
     const uint32_t c = blockIdx.x * 32 + (threadIdx.x & 31u), q = threadIdx.x >> 5, half = blockIdx.y;
     float s = 0.0f;
@@ -283,7 +289,7 @@ static uint32_t norm_group(uint32_t cols, uint32_t values) {
 template <typename T, int VEC, int G>
 static void norm_launch(void *y, float *mean, float *rstd, const void *x, const void *gamma, const void *beta, uint32_t rows, uint32_t cols, float eps) {
     const uint32_t per = G > 32 ? 1 : NORM_BLOCK / 32;
-    k_norm<T, VEC, G><<<(rows + per - 1) / per, G > 32 ? G : NORM_BLOCK, 0, g.stream>>>((T *)y, mean, rstd, (const T *)x, (const T *)gamma, (const T *)beta, rows, cols, eps);
+    chain(k_norm<T, VEC, G>, dim3((rows + per - 1) / per), G > 32 ? G : NORM_BLOCK, 0, (T *)y, mean, rstd, (const T *)x, (const T *)gamma, (const T *)beta, rows, cols, eps);
 }
 template <typename T, int VEC>
 static void norm_launch_g(uint32_t group, void *y, float *mean, float *rstd, const void *x, const void *gamma, const void *beta, uint32_t rows, uint32_t cols, float eps) {
@@ -298,14 +304,14 @@ static void norm_launch_g(uint32_t group, void *y, float *mean, float *rstd, con
 template <typename T>
 static void norm_forward(void *y, float *mean, float *rstd, const void *x, const void *gamma, const void *beta, uint32_t rows, uint32_t cols, float eps) {
     const uint32_t group = norm_group(cols, NORM_VALUES);
-    if (!group) k_norm_long<T><<<grid_for(rows, 1, 2), 1024, 0, g.stream>>>((T *)y, mean, rstd, (const T *)x, (const T *)gamma, (const T *)beta, rows, cols, eps);
+    if (!group) chain(k_norm_long<T>, dim3(grid_for(rows, 1, 2)), 1024, 0, (T *)y, mean, rstd, (const T *)x, (const T *)gamma, (const T *)beta, rows, cols, eps);
     else if (cols % Vec16<T>::n == 0) norm_launch_g<T, Vec16<T>::n>(group, y, mean, rstd, x, gamma, beta, rows, cols, eps);
     else norm_launch_g<T, 1>(group, y, mean, rstd, x, gamma, beta, rows, cols, eps);
 }
 
 template <typename T, int VEC, int G>
 static void norm_bwd_launch(void *dx, float *partial, const void *dy, const void *x, const void *gamma, const float *mean, const float *rstd, uint32_t rows, uint32_t cols, uint32_t blocks) {
-    k_norm_bwd<T, VEC, G><<<blocks, G > 32 ? G : NORM_BLOCK, 0, g.stream>>>((T *)dx, partial, (const T *)dy, (const T *)x, (const T *)gamma, mean, rstd, rows, cols);
+    chain(k_norm_bwd<T, VEC, G>, dim3(blocks), G > 32 ? G : NORM_BLOCK, 0, (T *)dx, partial, (const T *)dy, (const T *)x, (const T *)gamma, mean, rstd, rows, cols);
 }
 template <typename T, int VEC>
 static void norm_bwd_launch_g(uint32_t group, void *dx, float *partial, const void *dy, const void *x, const void *gamma, const float *mean, const float *rstd, uint32_t rows, uint32_t cols, uint32_t blocks) {
@@ -335,18 +341,18 @@ static void norm_backward(void *dx, void *dgamma, void *dbeta, const void *dy, c
         n = rows < 16 ? rows : 16;
         if (sums) {                                    // first: dx may lie where dy or x does
             partial = (float *)scratch_reserve((uint64_t)n * 2 * cols * sizeof(float));
-            k_norm_bwd_cols<T><<<dim3((cols + 255) / 256, n), 256, 0, g.stream>>>(partial, (const T *)dy, (const T *)x, mean, rstd, rows, cols);
+            chain(k_norm_bwd_cols<T>, dim3((cols + 255) / 256, n), 256, 0, partial, (const T *)dy, (const T *)x, mean, rstd, rows, cols);
             after_launch("layernorm_backward_cols");
             profile_begin();
         }
         if (dx) {
-            k_norm_bwd_long<T><<<grid_for(rows, 1, 2), 1024, 0, g.stream>>>((T *)dx, (const T *)dy, (const T *)x, (const T *)gamma, mean, rstd, rows, cols);
+            chain(k_norm_bwd_long<T>, dim3(grid_for(rows, 1, 2)), 1024, 0, (T *)dx, (const T *)dy, (const T *)x, (const T *)gamma, mean, rstd, rows, cols);
             after_launch("layernorm_backward");
         }
     }
     if (sums) {
         profile_begin();
-        k_norm_fold<T><<<dim3((cols + 31) / 32, 2), 256, 0, g.stream>>>((T *)dgamma, (T *)dbeta, partial, n, cols);
+        chain(k_norm_fold<T>, dim3((cols + 31) / 32, 2), 256, 0, (T *)dgamma, (T *)dbeta, partial, n, cols);
         after_launch("layernorm_fold");
     }
 }

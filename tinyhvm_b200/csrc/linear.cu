@@ -89,6 +89,7 @@ __device__ __forceinline__ float block_max(float v, float *red) {
 template <class Src, int VEC, int U>
 __global__ void __launch_bounds__(256)
 k_split_rows(const Src src, const Planes out, uint32_t rows, uint32_t cols) {
+    depend();
     __shared__ float red[8];
     float sum[U][VEC];
 #pragma unroll
@@ -138,6 +139,7 @@ k_split_rows(const Src src, const Planes out, uint32_t rows, uint32_t cols) {
 template <class Src>
 __global__ void __launch_bounds__(256)
 k_split_long_rows(const Src src, const Planes out, uint32_t rows, uint32_t cols) {
+    depend();
     __shared__ float red[8];
     for (uint64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         float v[1], top = 0.0f;
@@ -158,6 +160,7 @@ k_split_long_rows(const Src src, const Planes out, uint32_t rows, uint32_t cols)
 template <class Src>
 __global__ void __launch_bounds__(256)
 k_grad_sums(const Src src, float *sums, uint32_t rows, uint32_t cols) {
+    depend();
     const uint32_t c = blockIdx.x * 256 + threadIdx.x;
     if (c >= cols) return;
     float v[1], s = 0.0f;
@@ -168,6 +171,7 @@ k_grad_sums(const Src src, float *sums, uint32_t rows, uint32_t cols) {
 template <typename T>
 __global__ void __launch_bounds__(256)
 k_fold_sums(T *out, const float *sums, uint32_t n, uint32_t cols) {
+    depend();
     __shared__ float red[8][33];
     const uint32_t c = blockIdx.x * 32 + (threadIdx.x & 31u), q = threadIdx.x >> 5;
     float s = 0.0f;
@@ -186,6 +190,7 @@ k_fold_sums(T *out, const float *sums, uint32_t n, uint32_t cols) {
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
 k_col_tops(const T *x, const int *shift, float *tops, uint32_t rows, uint32_t cols) {
+    depend();
     const uint32_t c = (blockIdx.x * 256 + threadIdx.x) * VEC;
     if (c >= cols) return;
     float top[VEC] = {};
@@ -202,6 +207,7 @@ k_col_tops(const T *x, const int *shift, float *tops, uint32_t rows, uint32_t co
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
 k_split_cols(const T *x, const int *shift, const float *tops, const Planes out, uint32_t rows, uint32_t cols) {
+    depend();
     const uint32_t c = (blockIdx.x * 256 + threadIdx.x) * VEC;
     if (c >= cols) return;
     float scale[VEC];
@@ -228,16 +234,16 @@ template <class Src>
 static void split_rows(const Src &src, const Planes &out, uint32_t rows, uint32_t cols, uint32_t blocks, const char *name) {
     profile_begin();
     if (cols > ROW_VALUES) {
-        if (out.hi) { k_split_long_rows<Src><<<grid_for(rows, 1, 8), 256, 0, g.stream>>>(src, out, rows, cols); after_launch(name); profile_begin(); }
-        if (out.sums) { k_grad_sums<Src><<<dim3((cols + 255) / 256, blocks), 256, 0, g.stream>>>(src, out.sums, rows, cols); after_launch(name); }
+        if (out.hi) { chain(k_split_long_rows<Src>, dim3(grid_for(rows, 1, 8)), 256, 0, src, out, rows, cols); after_launch(name); profile_begin(); }
+        if (out.sums) { chain(k_grad_sums<Src>, dim3((cols + 255) / 256, blocks), 256, 0, src, out.sums, rows, cols); after_launch(name); }
         return;
     }
     if (cols % 4 == 0) {
-        if (cols <= 1024) k_split_rows<Src, 4, 1><<<blocks, 256, 0, g.stream>>>(src, out, rows, cols);
-        else if (cols <= 4096) k_split_rows<Src, 4, 4><<<blocks, 256, 0, g.stream>>>(src, out, rows, cols);
-        else k_split_rows<Src, 4, 8><<<blocks, 256, 0, g.stream>>>(src, out, rows, cols);
-    } else if (cols <= 1024) k_split_rows<Src, 1, 4><<<blocks, 256, 0, g.stream>>>(src, out, rows, cols);
-    else k_split_rows<Src, 1, 32><<<blocks, 256, 0, g.stream>>>(src, out, rows, cols);
+        if (cols <= 1024) chain(k_split_rows<Src, 4, 1>, dim3(blocks), 256, 0, src, out, rows, cols);
+        else if (cols <= 4096) chain(k_split_rows<Src, 4, 4>, dim3(blocks), 256, 0, src, out, rows, cols);
+        else chain(k_split_rows<Src, 4, 8>, dim3(blocks), 256, 0, src, out, rows, cols);
+    } else if (cols <= 1024) chain(k_split_rows<Src, 1, 4>, dim3(blocks), 256, 0, src, out, rows, cols);
+    else chain(k_split_rows<Src, 1, 32>, dim3(blocks), 256, 0, src, out, rows, cols);
     after_launch(name);
 }
 static uint32_t split_blocks(uint32_t rows) { return grid_for(rows, 1, 6); }
@@ -334,7 +340,7 @@ static hg::Operand f16_operand(Cut &c, const __half *p, uint32_t rows, uint32_t 
 template <typename T>
 static void linear_forward(void *y, void *z, const void *x, const void *w, const void *bias, const void *residual, uint32_t M, uint32_t K, uint32_t N, uint32_t act) {
     constexpr bool F = sizeof(T) == 4;
-    const hg::Plan plan = hg::plan(M, N, K, true);
+    const hg::Plan plan = hg::plan(M, N, K, false);
     const int *exps = nullptr;
     Cut c;
     hg::Operand A{}, B{};
@@ -373,7 +379,7 @@ static void linear_backward(void *dx, void *dw, void *dbias, const void *dy, con
     const bool scaled = F || smooth;                   // dz needs planes: f32, or f16 times a slope that is neither 0 nor 1
     const bool as_is = !F && act == THC_ACT_NONE && N % 8 == 0;
     const GradOf<T> grad{(const T *)dy, (const T *)z, N, act};
-    const hg::Plan plan_x = hg::plan(M, K, N, true), plan_w = hg::plan(K, N, M, true);
+    const hg::Plan plan_x = hg::plan(M, K, N, false), plan_w = hg::plan(K, N, M, false);
     const uint32_t blocks = split_blocks(M), sum_rows = N > ROW_VALUES ? (M < 16 ? M : 16) : blocks, runs = col_runs(M, K);
     Cut c;
     for (int pass = 0; pass < 2; pass++) {
@@ -386,7 +392,7 @@ static void linear_backward(void *dx, void *dw, void *dbias, const void *dy, con
         if (pass && (pz.hi || pz.sums)) split_rows(grad, pz, M, N, N > ROW_VALUES && pz.sums ? sum_rows : blocks, "linear_backward_dz");
         if (pass && dbias) {
             profile_begin();
-            k_fold_sums<T><<<(N + 31) / 32, 256, 0, g.stream>>>((T *)dbias, pz.sums, sum_rows, N);
+            chain(k_fold_sums<T>, dim3((N + 31) / 32), 256, 0, (T *)dbias, pz.sums, sum_rows, N);
             after_launch("linear_backward_bias");
         }
         const hg::Operand dz_k = as_is ? hg::Operand{(const __half *)dy, N, 0, false} : operand(pz, false);
@@ -413,11 +419,11 @@ static void linear_backward(void *dx, void *dw, void *dbias, const void *dy, con
                     profile_begin();
                     const T *xs = (const T *)x;
                     if (K % 4 == 0) {
-                        k_col_tops<T, 4><<<dim3((K / 4 + 255) / 256, runs), 256, 0, g.stream>>>(xs, pz.exps, tops, M, K);
-                        k_split_cols<T, 4><<<dim3((K / 4 + 255) / 256, runs), 256, 0, g.stream>>>(xs, pz.exps, tops, px, M, K);
+                        chain(k_col_tops<T, 4>, dim3((K / 4 + 255) / 256, runs), 256, 0, xs, pz.exps, tops, M, K);
+                        chain(k_split_cols<T, 4>, dim3((K / 4 + 255) / 256, runs), 256, 0, xs, pz.exps, tops, px, M, K);
                     } else {
-                        k_col_tops<T, 1><<<dim3((K + 255) / 256, runs), 256, 0, g.stream>>>(xs, pz.exps, tops, M, K);
-                        k_split_cols<T, 1><<<dim3((K + 255) / 256, runs), 256, 0, g.stream>>>(xs, pz.exps, tops, px, M, K);
+                        chain(k_col_tops<T, 1>, dim3((K + 255) / 256, runs), 256, 0, xs, pz.exps, tops, M, K);
+                        chain(k_split_cols<T, 1>, dim3((K + 255) / 256, runs), 256, 0, xs, pz.exps, tops, px, M, K);
                     }
                     after_launch("layer_operand");
                 }

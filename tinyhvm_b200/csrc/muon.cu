@@ -23,6 +23,7 @@ constexpr float PLANE = 8192.0f;
 template <int VEC>
 __global__ void __launch_bounds__(256)
 k_muon_momentum(float *mom, const float *grad, double *partial, float mu, int nesterov, uint64_t n) {
+    depend();
     __shared__ double red[8];
     double s = 0.0;
     for (uint64_t i = (blockIdx.x * 256ull + threadIdx.x) * VEC; i < n; i += gridDim.x * 256ull * VEC) {
@@ -52,6 +53,7 @@ k_muon_momentum(float *mom, const float *grad, double *partial, float mu, int ne
 template <int VEC>
 __global__ void __launch_bounds__(256)
 k_muon_planes(__half *hi, __half *lo, uint64_t pitch, const float *mom, const float *grad, const double *partial, uint32_t n_partial, float mu, int nesterov, uint32_t rows, uint32_t cols) {
+    depend();
     __shared__ double red[8];
     __shared__ float inv;
     double s = 0.0;
@@ -163,8 +165,10 @@ static void newton_schulz(float *out, float *param, float *mom, const float *gra
     const uint32_t m = wide ? rows : cols, k = wide ? cols : rows;
     const uint64_t px = (cols + 63u) & ~63ull, pm = (m + 63u) & ~63ull, x_bytes = rows * px * 2, m_bytes = m * pm * 2;    // (multiples of 128)
     const unsigned blocks = grid_for(n, 1024, 4);
-    const hg::Plan square = hg::plan(m, m, k, false), poly = hg::plan(m, m, m, false), apply = hg::plan(rows, cols, m, true);
-    uint8_t *base = (uint8_t *)scratch_reserve(4 * x_bytes + 4 * m_bytes + apply.partial_bytes + blocks * sizeof(double));
+    const hg::Plan square = hg::plan(m, m, k, true), poly = hg::plan(m, m, m, true), apply = hg::plan(rows, cols, m, false);
+    uint64_t partial_bytes = square.partial_bytes > poly.partial_bytes ? square.partial_bytes : poly.partial_bytes;
+    if (apply.partial_bytes > partial_bytes) partial_bytes = apply.partial_bytes;
+    uint8_t *base = (uint8_t *)scratch_reserve(4 * x_bytes + 4 * m_bytes + ((partial_bytes + 7) & ~7ull) + blocks * sizeof(double));
     __half *x[2][2], *a[2], *b[2];
     for (int i = 0; i < 2; i++) {
         for (int p = 0; p < 2; p++) x[i][p] = (__half *)(base + (2 * i + p) * x_bytes);
@@ -172,20 +176,20 @@ static void newton_schulz(float *out, float *param, float *mom, const float *gra
         b[i] = (__half *)(base + 4 * x_bytes + (2 + i) * m_bytes);
     }
     float *partial = (float *)(base + 4 * x_bytes + 4 * m_bytes);
-    double *norms = (double *)(base + 4 * x_bytes + 4 * m_bytes + ((apply.partial_bytes + 7) & ~7ull));
+    double *norms = (double *)(base + 4 * x_bytes + 4 * m_bytes + ((partial_bytes + 7) & ~7ull));
     profile_begin();
-    if (n % 4 == 0) k_muon_momentum<4><<<blocks, 256, 0, g.stream>>>(mom, grad, norms, mu, nesterov, n);
-    else k_muon_momentum<1><<<blocks, 256, 0, g.stream>>>(mom, grad, norms, mu, nesterov, n);
+    if (n % 4 == 0) chain(k_muon_momentum<4>, dim3(blocks), 256, 0, mom, grad, norms, mu, nesterov, n);
+    else chain(k_muon_momentum<1>, dim3(blocks), 256, 0, mom, grad, norms, mu, nesterov, n);
     after_launch("newton_schulz_norm");
     profile_begin();
-    if (cols % 4 == 0) k_muon_planes<4><<<blocks, 256, 0, g.stream>>>(x[0][0], x[0][1], px, mom, grad, norms, blocks, mu, nesterov, rows, cols);
-    else k_muon_planes<1><<<blocks, 256, 0, g.stream>>>(x[0][0], x[0][1], px, mom, grad, norms, blocks, mu, nesterov, rows, cols);
+    if (cols % 4 == 0) chain(k_muon_planes<4>, dim3(blocks), 256, 0, x[0][0], x[0][1], px, mom, grad, norms, blocks, mu, nesterov, rows, cols);
+    else chain(k_muon_planes<1>, dim3(blocks), 256, 0, x[0][0], x[0][1], px, mom, grad, norms, blocks, mu, nesterov, rows, cols);
     after_launch("newton_schulz_planes");
     for (uint32_t i = 0; i < steps; i++) {
         __half **cur = x[i & 1], **next = x[(i & 1) ^ 1];
         const hg::Operand X{cur[0], px, rows * px, !wide}, A{a[0], pm, m * pm, false}, B{b[0], pm, m * pm, false};
-        hg::product(X, X, m, m, k, square, nullptr, SquareEpi{a[0], a[1], pm, m}, true, "newton_schulz_square");
-        hg::product(A, A, m, m, m, poly, nullptr, PolyEpi{b[0], b[1], a[0], a[1], pm, m}, true, "newton_schulz_poly");
+        hg::product(X, X, m, m, k, square, partial, SquareEpi{a[0], a[1], pm, m}, true, "newton_schulz_square");
+        hg::product(A, A, m, m, m, poly, partial, PolyEpi{b[0], b[1], a[0], a[1], pm, m}, true, "newton_schulz_poly");
         const hg::Operand Xr{cur[0], px, rows * px, wide};                     // X across: the other way round than in its square
         const auto run = [&](auto epi) { hg::product(wide ? B : Xr, wide ? Xr : B, rows, cols, m, apply, partial, epi, false, "newton_schulz_apply"); };
         if (i + 1 < steps) run(ApplyEpi<NEXT>{next[0], next[1], px, nullptr, cols, 0.0f, 0.0f});
