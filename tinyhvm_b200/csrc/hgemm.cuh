@@ -541,18 +541,26 @@ static uint32_t count_tiles(uint32_t M, uint32_t N, uint32_t nt, bool upper) {
     if (upper) { n = 0; for (uint32_t r = 0; r < rows; r++) n += cols - r * 256 / nt; }
     return n;
 }
-// Tile width and splits for an M x N product over K.  Wide tiles halve the traffic of A's panels, but a grid that leaves
-// pairs idle loses more: narrow ones then, and below half a grid K is split as well, into runs of at least 512 (the sums of a split
-// go through memory and a second kernel, some 5 us, which is what the products of 1024 k take).
-static Plan plan(uint32_t M, uint32_t N, uint32_t K, bool upper) {
-    const uint32_t pairs = (uint32_t)g.sm_count / 2;
-    Plan p;
-    p.nt = count_tiles(M, N, 256, upper) >= pairs ? 256 : 128;
-    const uint32_t tiles = count_tiles(M, N, p.nt, upper), most = K / 512;
-    p.splits = pairs / tiles < most ? pairs / tiles : most;
-    if (p.splits < 1) p.splits = 1;
-    p.partial_bytes = p.splits > 1 ? (uint64_t)p.splits * M * N * 4 : 0;
-    return p;
+// Tile width and splits over K for an M x N product: the least time in cycles by what the parts of one cost, measured.  A block of 64 k
+// with planes on both sides takes a pair 1900 cycles at 256 columns and 1500 at 128 (where issuing the MMAs is what takes long), one of
+// 128 k without planes 1550 and 1200; a tile's epilogue, as far as the next tile does not hide it, 4000 and 2000; the second kernel
+// that a split needs 5000, and the split's sums 3500 bytes a cycle, written and read.  4096 x 1024 x 4096: 64 wide tiles, 76 us; 128
+// narrow ones in two rounds, 137 us.
+static Plan plan(uint32_t M, uint32_t N, uint32_t K, bool planes, bool upper) {
+    const uint32_t pairs = (uint32_t)g.sm_count / 2, blocks = (K + (planes ? 63 : 127)) / (planes ? 64 : 128);
+    Plan best{256, 1, 0};
+    double least = 0;
+    for (uint32_t nt = 256; nt >= 128; nt -= 128) {
+        const uint32_t tiles = count_tiles(M, N, nt, upper);
+        const double block = planes ? (nt == 256 ? 1900 : 1500) : (nt == 256 ? 1550 : 1200), end = nt == 256 ? 4000 : 2000;
+        for (uint32_t s = 1; s <= 16 && (s == 1 || 2 * s <= blocks); s++) {
+            const double rounds = (double)(((uint64_t)tiles * s + pairs - 1) / pairs);
+            double t = rounds * (((blocks + s - 1) / s) * block + end);
+            if (s > 1) t += 5000 + (double)s * M * N * (upper ? 4.5 : 8) / 3500;
+            if (least == 0 || t < least) { least = t; best = Plan{nt, s, s > 1 ? (uint64_t)s * M * N * 4 : 0}; }
+        }
+    }
+    return best;
 }
 
 template <uint32_t NT, class Epi>

@@ -72,7 +72,10 @@ template <typename T> struct GradOf {                  // dz = dy act'(z)
     }
 };
 
-struct Planes { __half *hi, *lo; uint64_t pitch; int *exps; float *sums; };   // any of hi, lo, exps, sums may be null; exps null: unscaled
+struct Planes {
+    __half *hi, *lo; uint64_t pitch; int *exps; float *sums;       // any may be null; exps null: unscaled
+    uint32_t *clear; uint32_t n_clear;                             // words to be zeroed for a later kernel
+};
 
 __device__ __forceinline__ float block_max(float v, float *red) {
 #pragma unroll
@@ -91,6 +94,7 @@ __global__ void __launch_bounds__(256)
 k_split_rows(const Src src, const Planes out, uint32_t rows, uint32_t cols) {
     depend();
     __shared__ float red[8];
+    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < out.n_clear; i += gridDim.x * 256) out.clear[i] = 0;
     float sum[U][VEC];
 #pragma unroll
     for (int i = 0; i < U; i++)
@@ -141,6 +145,7 @@ __global__ void __launch_bounds__(256)
 k_split_long_rows(const Src src, const Planes out, uint32_t rows, uint32_t cols) {
     depend();
     __shared__ float red[8];
+    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < out.n_clear; i += gridDim.x * 256) out.clear[i] = 0;
     for (uint64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         float v[1], top = 0.0f;
         for (uint32_t c = threadIdx.x; c < cols; c += 256) { src.template load<1>(row, c, v); top = fmaxf(top, finite_abs(v[0])); }
@@ -186,14 +191,16 @@ k_fold_sums(T *out, const float *sums, uint32_t n, uint32_t cols) {
     }
 }
 
-// Scales by columns: the largest of x 2^-shift[row] over a run of rows, then the planes of it.
+// Scales by columns: the largest |x 2^-shift[row]| of each column, as bits (which order as the values do, so the order of the atomics does
+// not matter), then the planes.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
-k_col_tops(const T *x, const int *shift, float *tops, uint32_t rows, uint32_t cols) {
+k_col_tops(const T *x, const int *shift, uint32_t *tops, uint32_t rows, uint32_t cols) {
     depend();
     const uint32_t c = (blockIdx.x * 256 + threadIdx.x) * VEC;
     if (c >= cols) return;
     float top[VEC] = {};
+#pragma unroll 4
     for (uint64_t row = blockIdx.y; row < rows; row += gridDim.y) {
         float v[VEC];
         load_vec<VEC>(x + row * cols + c, v);
@@ -202,23 +209,22 @@ k_col_tops(const T *x, const int *shift, float *tops, uint32_t rows, uint32_t co
         for (int j = 0; j < VEC; j++) top[j] = fmaxf(top[j], finite_abs(v[j] * f));
     }
 #pragma unroll
-    for (int j = 0; j < VEC; j++) tops[(uint64_t)blockIdx.y * cols + c + j] = top[j];
+    for (int j = 0; j < VEC; j++) atomicMax(tops + c + j, __float_as_uint(top[j]));
 }
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
-k_split_cols(const T *x, const int *shift, const float *tops, const Planes out, uint32_t rows, uint32_t cols) {
+k_split_cols(const T *x, const int *shift, const uint32_t *tops, const Planes out, uint32_t rows, uint32_t cols) {
     depend();
     const uint32_t c = (blockIdx.x * 256 + threadIdx.x) * VEC;
     if (c >= cols) return;
     float scale[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; j++) {
-        float top = 0.0f;
-        for (uint32_t i = 0; i < gridDim.y; i++) top = fmaxf(top, tops[(uint64_t)i * cols + c + j]);
-        const int s = scale_for(top);
+        const int s = scale_for(__uint_as_float(tops[c + j]));
         if (blockIdx.y == 0) out.exps[c + j] = s;
         scale[j] = pow2(s);
     }
+#pragma unroll 4
     for (uint64_t row = blockIdx.y; row < rows; row += gridDim.y) {
         float v[VEC];
         load_vec<VEC>(x + row * cols + c, v);
@@ -246,13 +252,12 @@ static void split_rows(const Src &src, const Planes &out, uint32_t rows, uint32_
     else chain(k_split_rows<Src, 1, 32>, dim3(blocks), 256, 0, src, out, rows, cols);
     after_launch(name);
 }
-static uint32_t split_blocks(uint32_t rows) { return grid_for(rows, 1, 6); }
-static uint32_t col_runs(uint32_t rows, uint32_t cols) {         // runs of rows that k_col_tops splits a column into
-    const uint32_t across = (cols + 1023) / 1024, most = (rows + 15) / 16;
-    uint32_t n = (uint32_t)g.sm_count * 4 / across;
-    if (n > 64) n = 64;
+static uint32_t split_blocks(uint32_t rows) { return rows < (1u << 30) ? rows : 1u << 30; }      // a row each
+static uint32_t col_runs(uint32_t rows, uint32_t cols, uint32_t vec) {      // every how many rows a thread of k_col_tops looks: about eight blocks an SM, eight rows a thread
+    const uint32_t across = (cols / vec + 255) / 256, most = (rows + 7) / 8;
+    uint32_t n = (uint32_t)g.sm_count * 8 / across;
     if (n > most) n = most;
-    return n ? n : 1;
+    return n < 1 ? 1 : n > 65535 ? 65535 : n;
 }
 
 // scratch of one call, cut into pieces
@@ -329,6 +334,124 @@ template <typename T, bool COLS> struct GradEpi {      // sum 2^(-exps[m] - col_
     }
 };
 
+// ---- few rows: the weights are what is read, once, and the arithmetic is the CUDA cores' ----
+// A cluster of eight blocks takes 32 V columns of w and all of K: each block an eighth of K, each of its eight warps every eighth row of that,
+// a lane V neighbouring columns of MR rows of x.  The warps' sums meet in shared memory, the blocks' in the cluster's, in a fixed order;
+// each block then finishes an eighth of the columns.  x comes through shared memory, FEW_K of its columns at a time.
+// Bound by memory: K N values once.  V = 4: a lane copies its own weights to shared memory, FEW_RING groups of four rows ahead (16 KB
+// of f16 or 32 KB of f32 in flight per block, and no registers: as plain loads the compiler kept two or three in flight, and 4096 x 4096 f32
+// times one row took 32 us).  V = 1, for rows of w that are not aligned to four values: plain loads.
+constexpr uint32_t FEW_K = 512, FEW_CLUSTER = 8, FEW_RING = 4;
+template <typename T, int MR, int V> static constexpr uint32_t few_smem() {
+    return FEW_K * MR * 4 + (V == 4 && 8 * FEW_RING * 4 * 32 * V * sizeof(T) > 8u * MR * 32 * V * 4 ? 8 * FEW_RING * 4 * 32 * V * (uint32_t)sizeof(T) : 8u * MR * 32 * V * 4);
+}
+template <typename T> __device__ __forceinline__ void copy4(uint32_t dst, const T *src) {
+    if constexpr (sizeof(T) == 4) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+template <typename T, int MR, int V>
+__global__ void __cluster_dims__(1, FEW_CLUSTER, 1) __launch_bounds__(256)
+k_linear_few(T *y, T *z, const T *x, const T *w, const T *bias, const T *residual, uint32_t M, uint32_t K, uint32_t N, uint32_t act) {
+    depend();
+    constexpr uint32_t COLS = 32 * V;
+    extern __shared__ float few[];
+    float (*xs)[MR] = reinterpret_cast<float (*)[MR]>(few);                      // [FEW_K]
+    float (*sums)[MR][COLS] = reinterpret_cast<float (*)[MR][COLS]>(few + FEW_K * MR);   // [8], where the ring was
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, rank = blockIdx.y % FEW_CLUSTER;
+    const uint32_t n = blockIdx.x * COLS + lane * V, m0 = blockIdx.y / FEW_CLUSTER * MR;
+    const uint32_t share = (K + FEW_CLUSTER - 1) / FEW_CLUSTER, k_begin = rank * share < K ? rank * share : K, k_end = k_begin + share < K ? k_begin + share : K;
+    const uint64_t down = (uint64_t)8 * N;
+    // this lane's place in its warp's ring: row r of group g at + (g * 4 + r) * COLS values
+    const T *ring = reinterpret_cast<const T *>(few + FEW_K * MR) + warp * (FEW_RING * 4 * COLS) + lane * V;
+    float acc[MR][V];
+#pragma unroll
+    for (int i = 0; i < MR; i++)
+#pragma unroll
+        for (int j = 0; j < V; j++) acc[i][j] = 0.0f;
+    for (uint32_t k0 = k_begin; k0 < k_end; k0 += FEW_K) {
+        const uint32_t nk = k_end - k0 < FEW_K ? k_end - k0 : FEW_K;
+        const uint32_t mine = n < N && warp < nk ? (nk - warp + 7) / 8 : 0;           // rows k0 + warp + 8 i
+        const T *p = w + (uint64_t)(k0 + warp) * N + n;
+        if constexpr (V == 4) {
+#pragma unroll
+            for (uint32_t gr = 0; gr < FEW_RING - 1; gr++) {
+#pragma unroll
+                for (uint32_t r = 0; r < 4; r++) if (gr * 4 + r < mine) copy4(hg::smem32(ring + (gr * 4 + r) * COLS), p + (gr * 4 + r) * down);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            }
+        }
+        __syncthreads();
+        for (uint32_t u = threadIdx.x; u < MR * FEW_K; u += 256) {
+            const uint32_t i = u / FEW_K, k = u % FEW_K;
+            if (k < nk) xs[k][i] = m0 + i < M ? to_f32(x[(uint64_t)(m0 + i) * K + k0 + k]) : 0.0f;
+        }
+        __syncthreads();
+        if constexpr (V == 4) {
+            for (uint32_t i0 = 0, at = 0; i0 < mine; i0 += 4, at = (at + 1) % FEW_RING) {
+                const uint32_t ahead = i0 + 4 * (FEW_RING - 1), to = (at + FEW_RING - 1) % FEW_RING;
+#pragma unroll
+                for (uint32_t r = 0; r < 4; r++) if (ahead + r < mine) copy4(hg::smem32(ring + (to * 4 + r) * COLS), p + (ahead + r) * down);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                asm volatile("cp.async.wait_group %0;" ::"n"(FEW_RING - 1) : "memory");
+#pragma unroll
+                for (uint32_t r = 0; r < 4; r++) {
+                    if (i0 + r >= mine) break;
+                    float v[V];
+                    load_vec<V>(ring + (at * 4 + r) * COLS, v);
+                    const float *xk = xs[warp + 8 * (i0 + r)];
+#pragma unroll
+                    for (int i = 0; i < MR; i++)
+#pragma unroll
+                        for (int j = 0; j < V; j++) acc[i][j] += xk[i] * v[j];
+                }
+            }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+        } else {
+#pragma unroll 8
+            for (uint32_t i0 = 0; i0 < mine; i0++) {
+                const float v = to_f32(p[i0 * down]);
+                const float *xk = xs[warp + 8 * i0];
+#pragma unroll
+                for (int i = 0; i < MR; i++) acc[i][0] += xk[i] * v;
+            }
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MR; i++)
+#pragma unroll
+        for (int j = 0; j < V; j++) sums[warp][i][lane * V + j] = acc[i][j];
+    __syncthreads();
+    for (uint32_t u = threadIdx.x; u < MR * COLS; u += 256) {
+        const uint32_t i = u / COLS, c = u % COLS;
+        float s = sums[0][i][c];
+#pragma unroll
+        for (int q = 1; q < 8; q++) s += sums[q][i][c];
+        sums[0][i][c] = s;
+    }
+    hg::cluster_sync();
+    constexpr uint32_t MINE = COLS / FEW_CLUSTER;
+    for (uint32_t u = threadIdx.x; u < MR * MINE; u += 256) {
+        const uint32_t i = u / MINE, c = rank * MINE + u % MINE, col = blockIdx.x * COLS + c, m = m0 + i;
+        const uint32_t here = hg::smem32(&sums[0][i][c]);
+        float s = 0.0f;
+#pragma unroll
+        for (uint32_t r = 0; r < FEW_CLUSTER; r++) {
+            float q;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(q) : "r"(hg::in_cta(here, r)) : "memory");
+            s += q;
+        }
+        if (col >= N || m >= M) continue;
+        const uint64_t at = (uint64_t)m * N + col;
+        if (bias) s += to_f32(bias[col]);
+        if (z) put_f32(z + at, s);
+        s = act_value(act, s);
+        if (residual) s += to_f32(residual[at]);
+        put_f32(y + at, s);
+    }
+    hg::cluster_sync();                                // no block leaves while another reads its sums
+}
+
 // an f16 matrix as it is, or copied to a pitch that tile loads can take
 static hg::Operand f16_operand(Cut &c, const __half *p, uint32_t rows, uint32_t cols, bool mn, bool copy) {
     if (cols % 8 == 0) return hg::Operand{p, cols, 0, mn};
@@ -337,10 +460,36 @@ static hg::Operand f16_operand(Cut &c, const __half *p, uint32_t rows, uint32_t 
     return operand(q, mn);
 }
 
+template <typename T, int MR, int V>
+static void few_rows_as(void *y, void *z, const void *x, const void *w, const void *bias, const void *residual, uint32_t M, uint32_t K, uint32_t N, uint32_t act) {
+    static bool ready = false;
+    if (!ready) { THC_CUDA_OK(cudaFuncSetAttribute(k_linear_few<T, MR, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)few_smem<T, MR, V>())); ready = true; }
+    chain(k_linear_few<T, MR, V>, dim3((N + 32 * V - 1) / (32 * V), (M + MR - 1) / MR * FEW_CLUSTER), 256, few_smem<T, MR, V>(), (T *)y, (T *)z, (const T *)x, (const T *)w, (const T *)bias, (const T *)residual, M, K, N, act);
+}
+// Up to how many rows the kernel above is taken, from 4096 x 4096 weights.  f32: 15 us for one row, 19 for eight, 37 for 16, 53 for 24, 68 for 32;
+// the matrix engine, which splits the weights into planes first, 65 whatever the rows up to 128.  f16: 11 us for one row, 14 for
+// four, 18 for eight; the engine 18.  Where rows of w are not aligned, the engine copies them first: 16 rows for either type.
+template <typename T> static bool few_rows(void *y, void *z, const void *x, const void *w, const void *bias, const void *residual, uint32_t M, uint32_t K, uint32_t N, uint32_t act) {
+    profile_begin();
+    if (N % 4) {
+        if (M > 16) return false;
+        if (M <= 2) few_rows_as<T, 2, 1>(y, z, x, w, bias, residual, M, K, N, act);
+        else few_rows_as<T, 8, 1>(y, z, x, w, bias, residual, M, K, N, act);
+    } else {
+        if (M > (sizeof(T) == 4 ? 24 : 4)) return false;
+        if (M == 1) few_rows_as<T, 1, 4>(y, z, x, w, bias, residual, M, K, N, act);
+        else if (M <= 4) few_rows_as<T, 4, 4>(y, z, x, w, bias, residual, M, K, N, act);
+        else if constexpr (sizeof(T) == 4) few_rows_as<T, 8, 4>(y, z, x, w, bias, residual, M, K, N, act);
+    }
+    after_launch("linear_few");
+    return true;
+}
+
 template <typename T>
 static void linear_forward(void *y, void *z, const void *x, const void *w, const void *bias, const void *residual, uint32_t M, uint32_t K, uint32_t N, uint32_t act) {
     constexpr bool F = sizeof(T) == 4;
-    const hg::Plan plan = hg::plan(M, N, K, false);
+    if (few_rows<T>(y, z, x, w, bias, residual, M, K, N, act)) return;
+    const hg::Plan plan = hg::plan(M, N, K, F, false);
     const int *exps = nullptr;
     Cut c;
     hg::Operand A{}, B{};
@@ -379,8 +528,8 @@ static void linear_backward(void *dx, void *dw, void *dbias, const void *dy, con
     const bool scaled = F || smooth;                   // dz needs planes: f32, or f16 times a slope that is neither 0 nor 1
     const bool as_is = !F && act == THC_ACT_NONE && N % 8 == 0;
     const GradOf<T> grad{(const T *)dy, (const T *)z, N, act};
-    const hg::Plan plan_x = hg::plan(M, K, N, false), plan_w = hg::plan(K, N, M, false);
-    const uint32_t blocks = split_blocks(M), sum_rows = N > ROW_VALUES ? (M < 16 ? M : 16) : blocks, runs = col_runs(M, K);
+    const hg::Plan plan_x = hg::plan(M, K, N, scaled, false), plan_w = hg::plan(K, N, M, scaled, false);
+    const uint32_t blocks = dbias ? grid_for(M, 1, 2) : split_blocks(M), sum_rows = N > ROW_VALUES ? (M < 16 ? M : 16) : blocks;
     Cut c;
     for (int pass = 0; pass < 2; pass++) {
         if (pass) { c.base = (uint8_t *)scratch_reserve(c.at); c.at = 0; }
@@ -388,6 +537,7 @@ static void linear_backward(void *dx, void *dw, void *dbias, const void *dy, con
         // dz, and its sums over rows
         Planes pz{};
         if (!as_is && (dx || dw)) pz = take_planes(c, M, N, scaled, scaled, M);
+        if (scaled && dw) { pz.clear = c.take<uint32_t>(K); pz.n_clear = K; }
         pz.sums = dbias ? c.take<float>((uint64_t)sum_rows * N) : nullptr;
         if (pass && (pz.hi || pz.sums)) split_rows(grad, pz, M, N, N > ROW_VALUES && pz.sums ? sum_rows : blocks, "linear_backward_dz");
         if (pass && dbias) {
@@ -414,16 +564,17 @@ static void linear_backward(void *dx, void *dw, void *dbias, const void *dy, con
             const int *exps = nullptr;
             if (scaled) {                              // x takes dz's scales back
                 const Planes px = take_planes(c, M, K, F, true, K);
-                float *tops = c.take<float>((uint64_t)runs * K);
                 if (pass) {
-                    profile_begin();
                     const T *xs = (const T *)x;
-                    if (K % 4 == 0) {
-                        chain(k_col_tops<T, 4>, dim3((K / 4 + 255) / 256, runs), 256, 0, xs, pz.exps, tops, M, K);
-                        chain(k_split_cols<T, 4>, dim3((K / 4 + 255) / 256, runs), 256, 0, xs, pz.exps, tops, px, M, K);
+                    const uint32_t vec = K % 4 == 0 ? 4 : 1;
+                    const dim3 grid((K / vec + 255) / 256, col_runs(M, K, vec));
+                    profile_begin();
+                    if (vec == 4) {
+                        chain(k_col_tops<T, 4>, grid, 256, 0, xs, pz.exps, pz.clear, M, K);
+                        chain(k_split_cols<T, 4>, grid, 256, 0, xs, pz.exps, pz.clear, px, M, K);
                     } else {
-                        chain(k_col_tops<T, 1>, dim3((K + 255) / 256, runs), 256, 0, xs, pz.exps, tops, M, K);
-                        chain(k_split_cols<T, 1>, dim3((K + 255) / 256, runs), 256, 0, xs, pz.exps, tops, px, M, K);
+                        chain(k_col_tops<T, 1>, grid, 256, 0, xs, pz.exps, pz.clear, M, K);
+                        chain(k_split_cols<T, 1>, grid, 256, 0, xs, pz.exps, pz.clear, px, M, K);
                     }
                     after_launch("layer_operand");
                 }

@@ -165,7 +165,7 @@ static void newton_schulz(float *out, float *param, float *mom, const float *gra
     const uint32_t m = wide ? rows : cols, k = wide ? cols : rows;
     const uint64_t px = (cols + 63u) & ~63ull, pm = (m + 63u) & ~63ull, x_bytes = rows * px * 2, m_bytes = m * pm * 2;    // (multiples of 128)
     const unsigned blocks = grid_for(n, 1024, 4);
-    const hg::Plan square = hg::plan(m, m, k, true), poly = hg::plan(m, m, m, true), apply = hg::plan(rows, cols, m, false);
+    const hg::Plan square = hg::plan(m, m, k, true, true), poly = hg::plan(m, m, m, true, true), apply = hg::plan(rows, cols, m, true, false);
     uint64_t partial_bytes = square.partial_bytes > poly.partial_bytes ? square.partial_bytes : poly.partial_bytes;
     if (apply.partial_bytes > partial_bytes) partial_bytes = apply.partial_bytes;
     uint8_t *base = (uint8_t *)scratch_reserve(4 * x_bytes + 4 * m_bytes + ((partial_bytes + 7) & ~7ull) + blocks * sizeof(double));
