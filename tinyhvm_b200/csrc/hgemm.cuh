@@ -173,8 +173,9 @@ template <uint32_t NT> __device__ __forceinline__ Tile tile_of(const Shape &S, u
 
 // Epi: what happens to finished sums, R rows (m, m + step, ...; those below M count) of V neighbouring columns at a time (V = 4 where
 // Epi::wide() says that the result's rows allow it, else 1).  column<V>(n) sets up what belongs to the columns n, n+1, ...; fetch<V>(m, n, x)
-// reads what a row's result needs from memory; row_factor(m), exact, goes onto a row's sums before all that; put<V, R>(rows, n, v, x, z) finishes and stores.  With Epi::mirrors, mirror<V, R> stores
-// the transposed place of a symmetric product: rows along n, V neighbouring values of m.
+// reads what a row's result needs from memory; row_factor(m), exact, goes onto a row's sums before all that; put<V, R>(rows, n, v, x, z) finishes the values
+// in v and stores them.  With Epi::mirrors, mirror<V, R> stores finished values in the transposed place of a symmetric product: rows along n,
+// V neighbouring values of m.
 struct Rows { uint32_t first, step, end; };             // end: 0xffffffff where the caller knows that all are valid
 
 // A block of 32 x 32 sums passes through shared memory, one warp's 4 KB, from "a lane holds a row" to "eight lanes hold a row" (or
@@ -186,13 +187,13 @@ struct Rows { uint32_t first, step, end; };             // end: 0xffffffff where
 // tile's epilogue took 18000 cycles, where the MMAs of K = 1024 take 8000 in f16.
 __device__ __forceinline__ uint32_t swap(uint32_t r) { return (r ^ (r >> 2)) & 7u; }
 template <int V, bool WHOLE, class Epi>
-__device__ __forceinline__ void put_block(Epi &e, const float *st, uint32_t lane, uint32_t m0, uint32_t n0, uint32_t rows, uint32_t N, uint32_t z) {
+__device__ __forceinline__ void put_block(Epi &e, float *st, uint32_t lane, uint32_t m0, uint32_t n0, uint32_t rows, uint32_t N, uint32_t z) {
     const uint32_t M = WHOLE ? 0xffffffffu : rows;
     if constexpr (V == 4) {
         const uint32_t ro = lane >> 3, n = n0 + (lane & 7u) * 4u, b = (lane & 7u) ^ ro;
         if (!WHOLE && n >= N) return;
         e.template column<4>(n);
-        const float *p = st + ro * 32u;
+        float *p = st + ro * 32u;
 #pragma unroll
         for (uint32_t t = 0; t < 8; t += 4) {          // row ro + 4 t: swap(ro + 4 t) = ro ^ (4 (t & 1)) ^ t
             float x[4][4], v[4][4];
@@ -205,6 +206,11 @@ __device__ __forceinline__ void put_block(Epi &e, const float *st, uint32_t lane
                 v[i][0] = q.x; v[i][1] = q.y; v[i][2] = q.z; v[i][3] = q.w;
             }
             e.template put<4, 4>(Rows{m0 + ro + 4 * t, 4, M}, n, v, x, z);
+            if constexpr (Epi::mirrors) {              // the finished values go back, for the mirror to store
+#pragma unroll
+                for (uint32_t i = 0; i < 4; i++)
+                    *reinterpret_cast<float4 *>(p + (t + i) * 128u + ((b ^ (((i & 1u) * 4u) ^ (t + i))) << 2)) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
+            }
         }
     } else {
         const uint32_t n = n0 + lane;
@@ -219,6 +225,10 @@ __device__ __forceinline__ void put_block(Epi &e, const float *st, uint32_t lane
                 v[i][0] = st[(r0 + i) * 32u + (((lane >> 2) ^ swap(r0 + i)) << 2) + (lane & 3u)];
             }
             e.template put<1, 4>(Rows{m0 + r0, 1, M}, n, v, x, z);
+            if constexpr (Epi::mirrors) {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; i++) st[(r0 + i) * 32u + (((lane >> 2) ^ swap(r0 + i)) << 2) + (lane & 3u)] = v[i][0];
+            }
         }
     }
 }
@@ -328,6 +338,7 @@ k_hgemm(const __grid_constant__ Shape S, const __grid_constant__ Maps maps, cons
                 else if (wide) put_block<4, false>(e, st, lane, m0, n1, S.M, S.N, T.z);
                 else put_block<1, false>(e, st, lane, m0, n1, S.M, S.N, T.z);
                 if constexpr (Epi::mirrors) {
+                    __syncwarp();
                     if (above) { if (wide) mirror_block<4>(e, st, lane, m0, n1, S.N); else mirror_block<1>(e, st, lane, m0, n1, S.N); }
                 }
             }
@@ -480,20 +491,25 @@ k_hgemm_fold_upper(const float *partial, uint32_t splits, uint32_t M, const __gr
     constexpr uint32_t PER = 32 / V;                       // threads a row
     for (uint32_t u = threadIdx.x; u < 32 * PER; u += 256) {
         const uint32_t r = u / PER, c = (u % PER) * V;
+        if (m0 + r >= M || n0 + c >= M) continue;
         float x[1][V], v[1][V];
-        if (m0 + r < M && n0 + c < M) {
 #pragma unroll
-            for (uint32_t j = 0; j < V; j++) v[0][j] = st[r][c + j];
-            e.template column<V>(n0 + c);
-            e.template fetch<V>(m0 + r, n0 + c, x[0]);
-            e.template put<V, 1>(Rows{m0 + r, 1, M}, n0 + c, v, x, 0);
-        }
-        if (blockIdx.x > blockIdx.y && n0 + r < M && m0 + c < M) {
+        for (uint32_t j = 0; j < V; j++) v[0][j] = st[r][c + j];
+        e.template column<V>(n0 + c);
+        e.template fetch<V>(m0 + r, n0 + c, x[0]);
+        e.template put<V, 1>(Rows{m0 + r, 1, M}, n0 + c, v, x, 0);
+#pragma unroll
+        for (uint32_t j = 0; j < V; j++) st[r][c + j] = v[0][j];
+    }
+    __syncthreads();
+    if (blockIdx.x > blockIdx.y)
+        for (uint32_t u = threadIdx.x; u < 32 * PER; u += 256) {
+            const uint32_t r = u / PER, c = (u % PER) * V;
+            float v[1][V];
 #pragma unroll
             for (uint32_t j = 0; j < V; j++) v[0][j] = st[c + j][r];
-            e.template mirror<V, 1>(Rows{n0 + r, 1, M}, m0 + c, v);
+            if (n0 + r < M && m0 + c < M) e.template mirror<V, 1>(Rows{n0 + r, 1, M}, m0 + c, v);
         }
-    }
 }
 
 // ---- host ----
@@ -544,7 +560,7 @@ static uint32_t count_tiles(uint32_t M, uint32_t N, uint32_t nt, bool upper) {
 // Tile width and splits over K for an M x N product: the least time in cycles by what the parts of one cost, measured.  A block of 64 k
 // with planes on both sides takes a pair 1900 cycles at 256 columns and 1500 at 128 (where issuing the MMAs is what takes long), one of
 // 128 k without planes 1550 and 1200; a tile's epilogue, as far as the next tile does not hide it, 4000 and 2000; the second kernel
-// that a split needs 5000, and the split's sums 3500 bytes a cycle, written and read.  4096 x 1024 x 4096: 64 wide tiles, 76 us; 128
+// that a split needs 9000, and the split's sums 3500 bytes a cycle, written and read.  4096 x 1024 x 4096: 64 wide tiles, 76 us; 128
 // narrow ones in two rounds, 137 us.
 static Plan plan(uint32_t M, uint32_t N, uint32_t K, bool planes, bool upper) {
     const uint32_t pairs = (uint32_t)g.sm_count / 2, blocks = (K + (planes ? 63 : 127)) / (planes ? 64 : 128);
@@ -556,7 +572,7 @@ static Plan plan(uint32_t M, uint32_t N, uint32_t K, bool planes, bool upper) {
         for (uint32_t s = 1; s <= 16 && (s == 1 || 2 * s <= blocks); s++) {
             const double rounds = (double)(((uint64_t)tiles * s + pairs - 1) / pairs);
             double t = rounds * (((blocks + s - 1) / s) * block + end);
-            if (s > 1) t += 5000 + (double)s * M * N * (upper ? 4.5 : 8) / 3500;
+            if (s > 1) t += 9000 + (double)s * M * N * (upper ? 4.5 : 8) / 3500;
             if (least == 0 || t < least) { least = t; best = Plan{nt, s, s > 1 ? (uint64_t)s * M * N * 4 : 0}; }
         }
     }

@@ -73,6 +73,27 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
+// Column sums of partial rows: partial[n][gridDim.y][cols] -> first (blockIdx.y 0) and second (1), 32 columns a block of 1024, every 32nd row a
+// thread, in a fixed order.
+template <typename T>
+__global__ void __launch_bounds__(1024)
+k_fold_rows(T *first, T *second, const float *partial, uint32_t n, uint32_t cols) {
+    depend();
+    __shared__ float red[32][33];
+    const uint32_t lane = threadIdx.x & 31u, q = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+    T *out = blockIdx.y ? second : first;
+    if (!out) return;
+    float s = 0.0f;
+    if (c < cols) {
+#pragma unroll 4
+        for (uint32_t i = q; i < n; i += 32) s += partial[((uint64_t)i * gridDim.y + blockIdx.y) * cols + c];
+    }
+    red[q][lane] = s;
+    __syncthreads();
+    s = warp_sum(red[lane][q]);                        // warp q: column q of the block
+    if (lane == 0 && blockIdx.x * 32 + q < cols) put_f32(out + blockIdx.x * 32 + q, s);
+}
+
 // ---- activations (thvm_cuda_linear): value and slope at z ----
 // Phi(z) = (1 + erf(z / sqrt 2)) / 2.  With t = |z| / sqrt 2, erfc(t) = 2^(-t p(t)); p is a polynomial of degree 7 fitted to
 // -log2(erfc(t)) / t over [0, 4] so that erf's error is least at its largest (1.6e-8, with f32 arithmetic 7.5e-8; beyond 4, where

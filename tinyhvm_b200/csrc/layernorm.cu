@@ -10,7 +10,7 @@
 // A row belongs to a group of G threads, which keeps it in registers from the load to the store, so the deviation from
 // the mean is summed in a second pass that costs no memory traffic.  The backward pass keeps, beside the row, the running
 // column sums of dy xh and dy: a thread sees the same columns of every row its block visits.  Each block leaves one
-// partial row of sums and k_norm_fold adds those in block order, so results do not depend on timing.
+// partial row of sums and k_fold_rows adds those in block order, so results do not depend on timing.
 #include "layer_common.cuh"
 #include "layer_host.h"
 #include "state.h"
@@ -46,24 +46,31 @@ template <int G> __device__ __forceinline__ float2 group_sum2(float a, float b, 
 }
 
 constexpr int NORM_BLOCK = 256;                        // threads of a block whose groups are single warps
-constexpr int NORM_VALUES = 32;                        // values of a row that a thread of the forward kernel holds
+// values of a row that a thread of the forward kernel holds: 32 where there are rows for all SMs, 8 where latency counts, with gamma and
+// beta read beside x
+constexpr int NORM_VALUES = 32, NORM_VALUES_FEW = 8;
 
 // Forward.  G threads a row; blocks of G threads, or of NORM_BLOCK / 32 warps with a row each.
-template <typename T, int VEC, int G>
+template <typename T, int VEC, int G, int VALUES>
 __global__ void __launch_bounds__(G > 32 ? G : NORM_BLOCK)
 k_norm(T *y, float *mean_out, float *rstd_out, const T *x, const T *gamma, const T *beta, uint32_t rows, uint32_t cols, float eps) {
     depend();
-    constexpr int NV = NORM_VALUES / VEC;
+    constexpr int NV = VALUES / VEC;
+    constexpr bool EARLY = VALUES == NORM_VALUES_FEW;
     __shared__ float red[G > 32 ? G / 32 : 1];
     const uint32_t t = G > 32 ? threadIdx.x : (threadIdx.x & 31u);
     const uint64_t row = G > 32 ? blockIdx.x : (uint64_t)blockIdx.x * (NORM_BLOCK / 32) + (threadIdx.x >> 5);
     if (row >= rows) return;                           // (whole warps, and only where a row is one warp's)
     const T *xr = x + row * cols;
-    float v[NV][VEC];
+    float v[NV][VEC], gm[EARLY ? NV : 1][VEC], bt[EARLY ? NV : 1][VEC];
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
         const uint32_t c = (t + (uint32_t)i * G) * VEC;
+        if constexpr (EARLY) {
+            if (gamma && c < cols) load_vec<VEC>(gamma + c, gm[i]);
+            if (beta && c < cols) load_vec<VEC>(beta + c, bt[i]);
+        }
         if (c < cols) load_vec<VEC>(xr + c, v[i]);
         else {
 #pragma unroll
@@ -88,14 +95,16 @@ k_norm(T *y, float *mean_out, float *rstd_out, const T *x, const T *gamma, const
     for (int i = 0; i < NV; i++) {
         const uint32_t c = (t + (uint32_t)i * G) * VEC;
         if (c >= cols) continue;
-        float gm[VEC], bt[VEC];
-        if (gamma) load_vec<VEC>(gamma + c, gm);
-        if (beta) load_vec<VEC>(beta + c, bt);
+        constexpr int AT = EARLY ? 1 : 0;
+        if constexpr (!EARLY) {
+            if (gamma) load_vec<VEC>(gamma + c, gm[0]);
+            if (beta) load_vec<VEC>(beta + c, bt[0]);
+        }
 #pragma unroll
         for (int j = 0; j < VEC; j++) {
             float o = v[i][j] * rstd;
-            if (gamma) o *= gm[j];
-            if (beta) o += bt[j];
+            if (gamma) o *= gm[AT * i][j];
+            if (beta) o += bt[AT * i][j];
             v[i][j] = o;
         }
         store_vec<VEC>(yr + c, v[i]);
@@ -257,27 +266,6 @@ k_norm_bwd_cols(float *partial, const T *dy, const T *x, const float *mean, cons
     partial[((uint64_t)blockIdx.y * 2 + 1) * cols + c] = sb;
 }
 
-// partial[n][2][cols] -> dgamma, dbeta: 32 columns a block, eight threads a column, in block order
-template <typename T>
-__global__ void __launch_bounds__(256)
-k_norm_fold(T *dgamma, T *dbeta, const float *partial, uint32_t n, uint32_t cols) {
-    depend();
-    __shared__ float red[8][33];
-    const uint32_t c = blockIdx.x * 32 + (threadIdx.x & 31u), q = threadIdx.x >> 5, half = blockIdx.y;
-    float s = 0.0f;
-    if (c < cols)
-        for (uint32_t i = q; i < n; i += 8) s += partial[((uint64_t)i * 2 + half) * cols + c];
-    red[q][threadIdx.x & 31u] = s;
-    __syncthreads();
-    if (q == 0 && c < cols) {
-        s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) s += red[i][threadIdx.x];
-        T *out = half ? dbeta : dgamma;
-        if (out) put_f32(out + c, s);
-    }
-}
-
 // ---- host ----
 // threads of a row's group when each holds `values` of it: 32, 128, 256, 512 or 1024; 0 = none holds the row
 static uint32_t norm_group(uint32_t cols, uint32_t values) {
@@ -286,27 +274,32 @@ static uint32_t norm_group(uint32_t cols, uint32_t values) {
     return 0;
 }
 
-template <typename T, int VEC, int G>
+template <typename T, int VEC, int G, int VALUES>
 static void norm_launch(void *y, float *mean, float *rstd, const void *x, const void *gamma, const void *beta, uint32_t rows, uint32_t cols, float eps) {
     const uint32_t per = G > 32 ? 1 : NORM_BLOCK / 32;
-    chain(k_norm<T, VEC, G>, dim3((rows + per - 1) / per), G > 32 ? G : NORM_BLOCK, 0, (T *)y, mean, rstd, (const T *)x, (const T *)gamma, (const T *)beta, rows, cols, eps);
+    chain(k_norm<T, VEC, G, VALUES>, dim3((rows + per - 1) / per), G > 32 ? G : NORM_BLOCK, 0, (T *)y, mean, rstd, (const T *)x, (const T *)gamma, (const T *)beta, rows, cols, eps);
 }
-template <typename T, int VEC>
+template <typename T, int VEC, int VALUES>
 static void norm_launch_g(uint32_t group, void *y, float *mean, float *rstd, const void *x, const void *gamma, const void *beta, uint32_t rows, uint32_t cols, float eps) {
     switch (group) {
-        case 32:   norm_launch<T, VEC, 32>(y, mean, rstd, x, gamma, beta, rows, cols, eps); break;
-        case 128:  norm_launch<T, VEC, 128>(y, mean, rstd, x, gamma, beta, rows, cols, eps); break;
-        case 256:  norm_launch<T, VEC, 256>(y, mean, rstd, x, gamma, beta, rows, cols, eps); break;
-        case 512:  norm_launch<T, VEC, 512>(y, mean, rstd, x, gamma, beta, rows, cols, eps); break;
-        default:   norm_launch<T, VEC, 1024>(y, mean, rstd, x, gamma, beta, rows, cols, eps); break;
+        case 32:   norm_launch<T, VEC, 32, VALUES>(y, mean, rstd, x, gamma, beta, rows, cols, eps); break;
+        case 128:  norm_launch<T, VEC, 128, VALUES>(y, mean, rstd, x, gamma, beta, rows, cols, eps); break;
+        case 256:  norm_launch<T, VEC, 256, VALUES>(y, mean, rstd, x, gamma, beta, rows, cols, eps); break;
+        case 512:  norm_launch<T, VEC, 512, VALUES>(y, mean, rstd, x, gamma, beta, rows, cols, eps); break;
+        default:   norm_launch<T, VEC, 1024, VALUES>(y, mean, rstd, x, gamma, beta, rows, cols, eps); break;
     }
 }
 template <typename T>
 static void norm_forward(void *y, float *mean, float *rstd, const void *x, const void *gamma, const void *beta, uint32_t rows, uint32_t cols, float eps) {
-    const uint32_t group = norm_group(cols, NORM_VALUES);
-    if (!group) chain(k_norm_long<T>, dim3(grid_for(rows, 1, 2)), 1024, 0, (T *)y, mean, rstd, (const T *)x, (const T *)gamma, (const T *)beta, rows, cols, eps);
-    else if (cols % Vec16<T>::n == 0) norm_launch_g<T, Vec16<T>::n>(group, y, mean, rstd, x, gamma, beta, rows, cols, eps);
-    else norm_launch_g<T, 1>(group, y, mean, rstd, x, gamma, beta, rows, cols, eps);
+    constexpr int V = Vec16<T>::n;
+    const uint32_t few = norm_group(cols, NORM_VALUES_FEW), group = norm_group(cols, NORM_VALUES);
+    const bool wide = cols % V == 0;
+    if (few && (uint64_t)rows * few <= (uint64_t)g.sm_count * 1024) {     // all rows at once, at half the GPU's threads
+        if (wide) norm_launch_g<T, V, NORM_VALUES_FEW>(few, y, mean, rstd, x, gamma, beta, rows, cols, eps);
+        else norm_launch_g<T, 1, NORM_VALUES_FEW>(few, y, mean, rstd, x, gamma, beta, rows, cols, eps);
+    } else if (!group) chain(k_norm_long<T>, dim3(grid_for(rows, 1, 2)), 1024, 0, (T *)y, mean, rstd, (const T *)x, (const T *)gamma, (const T *)beta, rows, cols, eps);
+    else if (wide) norm_launch_g<T, V, NORM_VALUES>(group, y, mean, rstd, x, gamma, beta, rows, cols, eps);
+    else norm_launch_g<T, 1, NORM_VALUES>(group, y, mean, rstd, x, gamma, beta, rows, cols, eps);
 }
 
 template <typename T, int VEC, int G>
@@ -332,7 +325,8 @@ static void norm_backward(void *dx, void *dgamma, void *dbeta, const void *dy, c
     profile_begin();
     if (group) {
         const uint32_t threads = group > 32 ? group : NORM_BLOCK, per = group > 32 ? 1 : NORM_BLOCK / 32;
-        n = grid_for(rows, per, 1024 / threads);       // 1024 threads an SM: the registers allow no more
+        // 1024 threads an SM: the registers allow no more; and four rows a group at least, for the sums' sake
+        n = grid_for((rows + 3) / 4, per, 1024 / threads);
         if (sums) partial = (float *)scratch_reserve((uint64_t)n * 2 * cols * sizeof(float));
         if (cols % Vec16<T>::n == 0) norm_bwd_launch_g<T, Vec16<T>::n>(group, dx, partial, dy, x, gamma, mean, rstd, rows, cols, n);
         else norm_bwd_launch_g<T, 1>(group, dx, partial, dy, x, gamma, mean, rstd, rows, cols, n);
@@ -352,7 +346,7 @@ static void norm_backward(void *dx, void *dgamma, void *dbeta, const void *dy, c
     }
     if (sums) {
         profile_begin();
-        chain(k_norm_fold<T>, dim3((cols + 31) / 32, 2), 256, 0, (T *)dgamma, (T *)dbeta, partial, n, cols);
+        chain(k_fold_rows<T>, dim3((cols + 31) / 32, 2), 1024, 0, (T *)dgamma, (T *)dbeta, (const float *)partial, n, cols);
         after_launch("layernorm_fold");
     }
 }

@@ -172,25 +172,6 @@ k_grad_sums(const Src src, float *sums, uint32_t rows, uint32_t cols) {
     for (uint64_t row = blockIdx.y; row < rows; row += gridDim.y) { src.template load<1>(row, c, v); s += v[0]; }
     sums[(uint64_t)blockIdx.y * cols + c] = s;
 }
-// sums[n][cols] -> out: 32 columns a block, eight threads a column, in block order
-template <typename T>
-__global__ void __launch_bounds__(256)
-k_fold_sums(T *out, const float *sums, uint32_t n, uint32_t cols) {
-    depend();
-    __shared__ float red[8][33];
-    const uint32_t c = blockIdx.x * 32 + (threadIdx.x & 31u), q = threadIdx.x >> 5;
-    float s = 0.0f;
-    if (c < cols) for (uint32_t i = q; i < n; i += 8) s += sums[(uint64_t)i * cols + c];
-    red[q][threadIdx.x & 31u] = s;
-    __syncthreads();
-    if (q == 0 && c < cols) {
-        s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) s += red[i][threadIdx.x];
-        put_f32(out + c, s);
-    }
-}
-
 // Scales by columns: the largest |x 2^-shift[row]| of each column, as bits (which order as the values do, so the order of the atomics does
 // not matter), then the planes.
 template <typename T, int VEC>
@@ -200,7 +181,7 @@ k_col_tops(const T *x, const int *shift, uint32_t *tops, uint32_t rows, uint32_t
     const uint32_t c = (blockIdx.x * 256 + threadIdx.x) * VEC;
     if (c >= cols) return;
     float top[VEC] = {};
-#pragma unroll 4
+#pragma unroll 8
     for (uint64_t row = blockIdx.y; row < rows; row += gridDim.y) {
         float v[VEC];
         load_vec<VEC>(x + row * cols + c, v);
@@ -253,9 +234,9 @@ static void split_rows(const Src &src, const Planes &out, uint32_t rows, uint32_
     after_launch(name);
 }
 static uint32_t split_blocks(uint32_t rows) { return rows < (1u << 30) ? rows : 1u << 30; }      // a row each
-static uint32_t col_runs(uint32_t rows, uint32_t cols, uint32_t vec) {      // every how many rows a thread of k_col_tops looks: about eight blocks an SM, eight rows a thread
+static uint32_t col_runs(uint32_t rows, uint32_t cols, uint32_t vec) {      // every how many rows a thread of k_col_tops looks: two blocks an SM, as the columns' maxima meet in atomics; eight rows a thread at least
     const uint32_t across = (cols / vec + 255) / 256, most = (rows + 7) / 8;
-    uint32_t n = (uint32_t)g.sm_count * 8 / across;
+    uint32_t n = (uint32_t)g.sm_count * 2 / across;
     if (n > most) n = most;
     return n < 1 ? 1 : n > 65535 ? 65535 : n;
 }
@@ -529,7 +510,7 @@ static void linear_backward(void *dx, void *dw, void *dbias, const void *dy, con
     const bool as_is = !F && act == THC_ACT_NONE && N % 8 == 0;
     const GradOf<T> grad{(const T *)dy, (const T *)z, N, act};
     const hg::Plan plan_x = hg::plan(M, K, N, scaled, false), plan_w = hg::plan(K, N, M, scaled, false);
-    const uint32_t blocks = dbias ? grid_for(M, 1, 2) : split_blocks(M), sum_rows = N > ROW_VALUES ? (M < 16 ? M : 16) : blocks;
+    const uint32_t blocks = dbias ? grid_for(M, 1, 4) : split_blocks(M), sum_rows = N > ROW_VALUES ? (M < 16 ? M : 16) : blocks;
     Cut c;
     for (int pass = 0; pass < 2; pass++) {
         if (pass) { c.base = (uint8_t *)scratch_reserve(c.at); c.at = 0; }
@@ -542,7 +523,7 @@ static void linear_backward(void *dx, void *dw, void *dbias, const void *dy, con
         if (pass && (pz.hi || pz.sums)) split_rows(grad, pz, M, N, N > ROW_VALUES && pz.sums ? sum_rows : blocks, "linear_backward_dz");
         if (pass && dbias) {
             profile_begin();
-            chain(k_fold_sums<T>, dim3((N + 31) / 32), 256, 0, (T *)dbias, pz.sums, sum_rows, N);
+            chain(k_fold_rows<T>, dim3((N + 31) / 32, 1), 1024, 0, (T *)dbias, (T *)nullptr, (const float *)pz.sums, sum_rows, N);
             after_launch("linear_backward_bias");
         }
         const hg::Operand dz_k = as_is ? hg::Operand{(const __half *)dy, N, 0, false} : operand(pz, false);

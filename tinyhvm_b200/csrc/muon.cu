@@ -102,8 +102,8 @@ struct SquareEpi {                                     // A = X X^T
     __device__ void touch(uint32_t, uint32_t, uint32_t) const {}
     template <int V> __device__ void column(uint32_t) const {}
     template <int V> __device__ void fetch(uint32_t, uint32_t, float (&)[V]) const {}
-    template <int V, int R> __device__ void put(hg::Rows r, uint32_t n, float (&v)[R][V], const float (&)[R][V], uint32_t) const { mirror<V, R>(r, n, v); }
-    template <int V, int R> __device__ void mirror(hg::Rows r, uint32_t m, float (&v)[R][V]) const { put_planes<V, R>(hi, lo, pitch, r, m, v); }
+    template <int V, int R> __device__ void put(hg::Rows r, uint32_t n, float (&v)[R][V], const float (&)[R][V], uint32_t) const { put_planes<V, R>(hi, lo, pitch, r, n, v); }
+    template <int V, int R> __device__ void mirror(hg::Rows r, uint32_t m, const float (&v)[R][V]) const { put_planes<V, R>(hi, lo, pitch, r, m, v); }
 };
 struct PolyEpi {                                       // a I + b A + c A A
     static constexpr bool mirrors = true;
@@ -126,12 +126,7 @@ struct PolyEpi {                                       // a I + b A + c A A
             for (int j = 0; j < V; j++) v[i][j] = NS_B * x[i][j] + NS_C * v[i][j] + (r.first + i * r.step == n + j ? NS_A * PLANE : 0.0f);
         put_planes<V, R>(hi, lo, pitch, r, n, v);
     }
-    template <int V, int R> __device__ void mirror(hg::Rows r, uint32_t m, float (&v)[R][V]) const {
-        float x[R][V];
-#pragma unroll
-        for (uint32_t i = 0; i < R; i++) if (r.first + i * r.step < r.end) fetch<V>(r.first + i * r.step, m, x[i]);
-        put<V, R>(r, m, v, x, 0);
-    }
+    template <int V, int R> __device__ void mirror(hg::Rows r, uint32_t m, const float (&v)[R][V]) const { put_planes<V, R>(hi, lo, pitch, r, m, v); }
 };
 enum { NEXT, RESULT, STEP };
 template <int TO> struct ApplyEpi {                    // X = (a I + b A + c A A) X: planes for the next step, the result, or the parameters' step
