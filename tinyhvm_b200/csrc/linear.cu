@@ -5,6 +5,7 @@
 #include "hgemm.cuh"
 #include "layer_common.cuh"
 #include "layer_host.h"
+#include "layer_small.cuh"
 #include "state.h"
 
 namespace thc {
@@ -466,10 +467,27 @@ template <typename T> static bool few_rows(void *y, void *z, const void *x, cons
     return true;
 }
 
+// Up to how many products (M K N) the one-launch kernels of layer_small.cuh are taken.  Forward, f32: 512 x 400 x 120 in 9 us, the engine with its
+// operands' planes 16; 512 x 512 x 512 in 20 and 18; in f16 the engine needs no planes and is as fast at 64 x 64 x 64 (6 us).  Backward:
+// f32 256^3 12 and 31 us, 512 x 400 x 120 22 and 35, 1024 x 400 x 120 44 and 37; f16 17 and 27, 29 and 30; with 2000 rows, over which dw sums,
+// 32 and 34, 49 and 32.
+constexpr double SMALL_FORWARD = 1e8, SMALL_BACKWARD_F32 = 4e7, SMALL_BACKWARD_F16 = 2e7;
+constexpr uint32_t SMALL_BACKWARD_ROWS = 1024;
+
 template <typename T>
 static void linear_forward(void *y, void *z, const void *x, const void *w, const void *bias, const void *residual, uint32_t M, uint32_t K, uint32_t N, uint32_t act) {
     constexpr bool F = sizeof(T) == 4;
     if (few_rows<T>(y, z, x, w, bias, residual, M, K, N, act)) return;
+    if constexpr (F) if ((double)M * K * N <= SMALL_FORWARD) {
+        Small<T> S{};
+        S.x = (const T *)x; S.w = (const T *)w; S.bias = (const T *)bias; S.residual = (const T *)residual; S.y = (T *)y; S.z_out = (T *)z;
+        S.M = M; S.K = K; S.N = N; S.act = act;
+        const uint32_t tiles = ((M + 31) / 32) * ((N + 31) / 32), ranks = small_ranks(tiles, K, 8);
+        profile_begin();
+        chain_cluster(ranks, k_small_forward<T>, dim3(tiles, ranks), 128, 0, S);
+        after_launch("linear_small");
+        return;
+    }
     const hg::Plan plan = hg::plan(M, N, K, F, false);
     const int *exps = nullptr;
     Cut c;
@@ -505,6 +523,18 @@ static void linear_forward(void *y, void *z, const void *x, const void *w, const
 template <typename T>
 static void linear_backward(void *dx, void *dw, void *dbias, const void *dy, const void *z, const void *x, const void *w, uint32_t M, uint32_t K, uint32_t N, uint32_t act) {
     constexpr bool F = sizeof(T) == 4;
+    if ((double)M * K * N <= (F ? SMALL_BACKWARD_F32 : SMALL_BACKWARD_F16) && M <= SMALL_BACKWARD_ROWS) {
+        Small<T> S{};
+        S.x = (const T *)x; S.w = (const T *)w; S.dy = (const T *)dy; S.z_in = (const T *)z; S.dx = (T *)dx; S.dw = (T *)dw; S.dbias = (T *)dbias;
+        S.M = M; S.K = K; S.N = N; S.act = act;
+        const uint32_t m = (M + 31) / 32, k = (K + 31) / 32, n = (N + 31) / 32, ranks = small_ranks((uint64_t)m * k + k * n, M > N ? M : N, 16);   // (whatever is asked for)
+        S.dx_tiles = dx ? m * k : 0;
+        const uint32_t tiles = S.dx_tiles + (dw ? k * n : dbias ? n : 0);      // the bias's gradient comes from dw's first row of tiles
+        profile_begin();
+        chain_cluster(ranks, k_small_backward<T>, dim3(tiles, ranks), 128, 0, S);
+        after_launch("linear_backward_small");
+        return;
+    }
     const bool smooth = act == THC_ACT_GELU || act == THC_ACT_SILU;
     const bool scaled = F || smooth;                   // dz needs planes: f32, or f16 times a slope that is neither 0 nor 1
     const bool as_is = !F && act == THC_ACT_NONE && N % 8 == 0;

@@ -153,11 +153,170 @@ template <int TO> struct ApplyEpi {                    // X = (a I + b A + c A A
     }
 };
 
+// ---- small matrices: one launch, everything in one cluster's shared memory ----
+// The smaller side is at most 128, the larger 32 times the cluster.  Block r of the cluster keeps every row of its own share of the larger
+// side's columns, X_r (stored column by column), and A and B whole.  A step: P_r = X_r X_r^T by each block; A = sum of P_r, an equal share
+// of rows by each block, written to all; B = a I + b A + c A A the same way; X_r = B X_r.  Three barriers of the cluster a step.  All in
+// f32 on the CUDA cores: 0.03 GFLOP a step at 400 x 120 is nothing; what bounds it is the latency of the shared-memory reads with two warps a
+// scheduler and of the exchange.  As 15 launches of the matrix engine the same step takes 164 us.
+constexpr uint32_t NS_SIDE = 128, NS_SHARE = 32, NS_PITCH = 132;
+constexpr size_t NS_SMEM = (size_t)(NS_SHARE + 2 * NS_SIDE) * NS_PITCH * 4;
+struct NsSmall { float *out, *param, *mom; const float *grad; uint32_t rows, cols, steps; int nesterov; float mu, keep, step; };
+
+__device__ __forceinline__ float4 remote4(const float *p, uint32_t rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(hg::in_cta(hg::smem32(p), rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ void remote4(float *p, uint32_t rank, float4 v) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(hg::in_cta(hg::smem32(p), rank)), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+__global__ void __launch_bounds__(256, 1)
+k_ns_small(const __grid_constant__ NsSmall S) {
+    depend();
+    extern __shared__ __align__(16) float ns[];
+    float (*X)[NS_PITCH] = reinterpret_cast<float (*)[NS_PITCH]>(ns);                              // [NS_SHARE]: column, row
+    float (*A)[NS_PITCH] = X + NS_SHARE, (*B)[NS_PITCH] = A + NS_SIDE;                             // [NS_SIDE]; B first holds P
+    __shared__ double red[8], norm;
+    const uint32_t ranks = gridDim.y, rank = blockIdx.y, tid = threadIdx.x;
+    const bool wide = S.rows <= S.cols;
+    const uint32_t m = wide ? S.rows : S.cols, n = wide ? S.cols : S.rows, share = (n + ranks - 1) / ranks;
+    const uint32_t c0 = rank * share, mine = c0 >= n ? 0 : n - c0 < share ? n - c0 : share;        // columns c0 .. c0 + mine
+    // the update, its place in memory and its sum of squares; rows and columns beyond the matrix are zeros
+    const auto place = [&](uint32_t c, uint32_t r) { return wide ? (uint64_t)r * S.cols + c0 + c : (uint64_t)(c0 + c) * S.cols + r; };
+    const auto each = [&](auto f) {                        // lanes along memory
+        for (uint32_t u = tid; u < NS_SHARE * NS_SIDE; u += 256) { const uint32_t c = wide ? u % NS_SHARE : u / NS_SIDE, r = wide ? u / NS_SHARE : u % NS_SIDE; f(c, r, c < mine && r < m); }
+    };
+    double sq = 0.0;
+    each([&](uint32_t c, uint32_t r, bool in) {
+        float v = 0.0f;
+        if (in) {
+            const uint64_t at = place(c, r);
+            v = S.grad[at];
+            if (S.mom) { const float g = v, q = S.mu * S.mom[at] + g; S.mom[at] = q; v = S.nesterov ? g + S.mu * q : q; }
+        }
+        X[c][r] = v;
+        sq += (double)v * v;
+    });
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+    if ((tid & 31) == 0) red[tid >> 5] = sq;
+    __syncthreads();
+    if (tid == 0) { double s = 0.0; for (int w = 0; w < 8; w++) s += red[w]; norm = s; }
+    hg::cluster_sync();
+    double total = 0.0;
+    for (uint32_t q = 0; q < ranks; q++) {
+        double d;
+        asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(d) : "r"(hg::in_cta(hg::smem32(&norm), q)) : "memory");
+        total += d;
+    }
+    const float inv = (float)(1.0 / (sqrt(total) + 1e-7));
+    each([&](uint32_t c, uint32_t r, bool) { X[c][r] *= inv; });
+    const uint32_t band = NS_SIDE / ranks;                 // rows of A and of B that this block makes
+    for (uint32_t step = 0; step < S.steps; step++) {
+        __syncthreads();
+        {   // P = X_r X_r^T: 8 x 8 sums a thread
+            const uint32_t r0 = (tid >> 4) * 8, q0 = (tid & 15u) * 4;          // rows r0 .., columns q0 .. and q0 + 64 ..
+            float acc[8][8] = {};
+            for (uint32_t k = 0; k < mine; k++) {
+                const float4 a0 = *reinterpret_cast<const float4 *>(&X[k][r0]), a1 = *reinterpret_cast<const float4 *>(&X[k][r0 + 4]);
+                const float4 b0 = *reinterpret_cast<const float4 *>(&X[k][q0]), b1 = *reinterpret_cast<const float4 *>(&X[k][q0 + 64]);
+                const float a[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w}, b[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) acc[i][j] += a[i] * b[j];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                *reinterpret_cast<float4 *>(&B[r0 + i][q0]) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+                *reinterpret_cast<float4 *>(&B[r0 + i][q0 + 64]) = make_float4(acc[i][4], acc[i][5], acc[i][6], acc[i][7]);
+            }
+        }
+        hg::cluster_sync();
+        for (uint32_t u = tid; u < band * 32; u += 256) {   // this block's rows of A, to every block
+            const uint32_t r = rank * band + u / 32, c = u % 32 * 4;
+            float4 s = make_float4(0, 0, 0, 0);
+#pragma unroll 8
+            for (uint32_t q = 0; q < ranks; q++) { const float4 v = remote4(&B[r][c], q); s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w; }
+#pragma unroll 8
+            for (uint32_t q = 0; q < ranks; q++) remote4(&A[r][c], q, s);
+        }
+        hg::cluster_sync();
+        for (uint32_t u = tid; u < band * 32; u += 256) {   // its rows of a I + b A + c A A
+            const uint32_t r = rank * band + u / 32, c = u % 32 * 4;
+            float4 s = make_float4(0, 0, 0, 0);
+#pragma unroll 8
+            for (uint32_t k = 0; k < NS_SIDE; k++) {
+                const float a = A[r][k];
+                const float4 b = *reinterpret_cast<const float4 *>(&A[k][c]);
+                s.x += a * b.x; s.y += a * b.y; s.z += a * b.z; s.w += a * b.w;
+            }
+            const float4 q = *reinterpret_cast<const float4 *>(&A[r][c]);
+            s.x = NS_B * q.x + NS_C * s.x + (r == c ? NS_A : 0.0f); s.y = NS_B * q.y + NS_C * s.y + (r == c + 1 ? NS_A : 0.0f);
+            s.z = NS_B * q.z + NS_C * s.z + (r == c + 2 ? NS_A : 0.0f); s.w = NS_B * q.w + NS_C * s.w + (r == c + 3 ? NS_A : 0.0f);
+#pragma unroll 8
+            for (uint32_t t = 0; t < ranks; t++) remote4(&B[r][c], t, s);
+        }
+        hg::cluster_sync();
+        {   // X_r = B X_r: 4 rows x 4 columns a thread; B is symmetric, so its rows are read as columns
+            const uint32_t r0 = (tid & 31u) * 4, q0 = (tid >> 5) * 4;
+            float acc[4][4] = {};
+            if (q0 < mine) {
+#pragma unroll 4
+                for (uint32_t k = 0; k < m; k++) {
+                    const float4 b = *reinterpret_cast<const float4 *>(&B[k][r0]);
+                    const float x[4] = {X[q0][k], X[q0 + 1][k], X[q0 + 2][k], X[q0 + 3][k]};
+#pragma unroll
+                    for (int j = 0; j < 4; j++) { acc[j][0] += b.x * x[j]; acc[j][1] += b.y * x[j]; acc[j][2] += b.z * x[j]; acc[j][3] += b.w * x[j]; }
+                }
+            }
+            __syncthreads();
+            if (q0 < mine)
+#pragma unroll
+                for (int j = 0; j < 4; j++) *reinterpret_cast<float4 *>(&X[q0 + j][r0]) = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
+        }
+    }
+    __syncthreads();
+    each([&](uint32_t c, uint32_t r, bool in) {
+        if (!in) return;
+        const uint64_t at = place(c, r);
+        if (S.param) S.param[at] = S.param[at] * S.keep - S.step * X[c][r];
+        else S.out[at] = X[c][r];
+    });
+    hg::cluster_sync();                                    // no block leaves while another may still write to it
+}
+// the cluster's size for a matrix, or 0 where it does not fit; 16 blocks need the GPU's consent
+static uint32_t ns_small_ranks(uint32_t m, uint32_t n) {
+    if (m > NS_SIDE || n > NS_SHARE * 16) return 0;
+    static int most = 0;
+    if (!most) {
+        most = 8;
+        THC_CUDA_OK(cudaFuncSetAttribute(k_ns_small, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)NS_SMEM));
+        THC_CUDA_OK(cudaFuncSetAttribute(k_ns_small, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        cudaLaunchConfig_t c{};
+        cudaLaunchAttribute a[1];
+        a[0].id = cudaLaunchAttributeClusterDimension;
+        a[0].val.clusterDim.x = 1; a[0].val.clusterDim.y = 16; a[0].val.clusterDim.z = 1;
+        c.gridDim = dim3(1, 16); c.blockDim = dim3(256); c.dynamicSmemBytes = NS_SMEM; c.attrs = a; c.numAttrs = 1;
+        int clusters = 0;
+        if (cudaOccupancyMaxActiveClusters(&clusters, k_ns_small, &c) == cudaSuccess && clusters > 0) most = 16;
+        else cudaGetLastError();
+    }
+    return n <= NS_SHARE * (uint32_t)most ? (uint32_t)most : 0;
+}
+
 // out (or the parameter step, when param is given) <- Newton-Schulz of grad or of the momentum update
 static void newton_schulz(float *out, float *param, float *mom, const float *grad, uint32_t rows, uint32_t cols, uint32_t steps, float mu, int nesterov, float keep, float step) {
     const uint64_t n = (uint64_t)rows * cols;
     const bool wide = rows <= cols;
     const uint32_t m = wide ? rows : cols, k = wide ? cols : rows;
+    if (const uint32_t ranks = ns_small_ranks(m, k)) {
+        profile_begin();
+        chain_cluster(ranks, k_ns_small, dim3(1, ranks), 256, NS_SMEM, NsSmall{out, param, mom, grad, rows, cols, steps, nesterov, mu, keep, step});
+        after_launch("newton_schulz_small");
+        return;
+    }
     const uint64_t px = (cols + 63u) & ~63ull, pm = (m + 63u) & ~63ull, x_bytes = rows * px * 2, m_bytes = m * pm * 2;    // (multiples of 128)
     const unsigned blocks = grid_for(n, 1024, 4);
     const hg::Plan square = hg::plan(m, m, k, true, true), poly = hg::plan(m, m, m, true, true), apply = hg::plan(rows, cols, m, true, false);
