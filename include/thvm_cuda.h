@@ -329,8 +329,11 @@ int      thvm_cuda_argmax_rows(uint32_t out_u32, uint32_t x, uint32_t rows, uint
  * dtype (THC_F32 or THC_F16); sums are f32 or wider, and f16 results are rounded to nearest even once, when stored.  Work
  * is queued on the backend's stream and can be recorded into a captured step.  All return 0 = launched, 1 = bad argument
  * with the reason in thvm_cuda_last_error() and nothing written: an empty shape, a missing, dead or too small buffer, an
- * unknown dtype or activation, or an output that is also an input or another output (exceptions below).  An id of 0 leaves an
- * optional operand out. */
+ * unknown dtype or activation, a dimension above 2^30, or an output that is also an input or another output (exceptions below).
+ * An id of 0 leaves an optional operand out.  Inside a captured step the same code means that library scratch had to grow: run
+ * the step once before capturing it.  f32 products keep f32's accuracy at the matrix engine's f16 rate (values are split in two); a value
+ * below 2^-40 of the largest in its row of x, w or dy (in dw: of x's column, each row of dy taken with its size) is rounded to
+ * that step, and an infinity in an f32 operand may give NaN where the sum would be infinite. */
 #define THC_ACT_NONE 0
 #define THC_ACT_RELU 1                  /* z > 0 ? z : 0, as the RELU op */
 #define THC_ACT_GELU 2                  /* z (1 + erf(z / sqrt 2)) / 2 */

@@ -21,7 +21,11 @@ NP = {F32: np.float32, F16: np.float16}
 HALF = {F32: 2.0 ** -24, F16: 2.0 ** -11}
 TINY = {F32: 2.0 ** -140, F16: 2.0 ** -25}
 NONE, RELU, GELU, SILU = range(4)
-erf = np.vectorize(math.erf)
+
+
+def erf(z):
+    import torch
+    return torch.erf(torch.from_numpy(np.ascontiguousarray(z))).numpy()
 
 
 # ---- definitions in 64 bits ----
@@ -199,7 +203,9 @@ def test_refusals_of_buffers(host):
 
 # ---- linear ----
 SHAPES = [(1, 1, 1), (1, 64, 8), (1, 513, 1000), (3, 40, 33), (7, 400, 120), (16, 257, 64), (17, 128, 264), (33, 784, 100), (64, 64, 64),
-          (100, 72, 200), (129, 65, 127), (128, 1000, 136), (200, 2056, 72), (300, 520, 513), (512, 400, 120), (257, 96, 1032), (1, 5000, 24), (40, 8, 3000)]
+          (100, 72, 200), (129, 65, 127), (128, 1000, 136), (200, 2056, 72), (300, 520, 513), (512, 400, 120), (257, 96, 1032), (1, 5000, 24), (40, 8, 3000),
+          # large enough for the matrix engine in f32 as well: ragged, aligned, split over K, long rows of w and of x
+          (301, 777, 701), (520, 640, 704), (130, 4104, 264), (1100, 264, 520), (70, 200, 9001), (50, 9000, 264), (24, 300, 200), (25, 512, 9000)]
 
 
 @pytest.mark.gpu
@@ -422,7 +428,7 @@ def test_layernorm_of_large_means_and_constant_rows(host):
 
 
 # ---- Newton-Schulz ----
-MATRICES = [(1, 1), (1, 50), (50, 1), (8, 8), (10, 84), (84, 10), (120, 84), (400, 120), (96, 97), (128, 256), (130, 520), (520, 264), (300, 300)]
+MATRICES = [(1, 1), (1, 50), (50, 1), (8, 8), (10, 84), (84, 10), (120, 84), (400, 120), (96, 97), (128, 256), (130, 520), (520, 264), (300, 300), (128, 512), (129, 400), (100, 513), (200, 2100), (1100, 150), (600, 601)]
 
 
 def spread(rng, rows, cols):
@@ -479,4 +485,166 @@ def test_newton_schulz_of_zeros(host):
     bx, bo = host.up(np.zeros((40, 30), np.float32)), host.out(1200)
     assert host.lib.thvm_cuda_newton_schulz(bo, bx, 40, 30, 5) == 0
     assert np.all(host.get(bo, 1200) == 0)
+    host.done()
+
+
+# ---- together, captured, and beside other work ----
+def layer_step(lib, b, dims, lr):
+    """Norm, layer, layer with residual, their gradients, and the optimizer on both weights: what one training step of such a block queues."""
+    M, D, H = dims
+    ok = lib.thvm_cuda_layernorm(b["n"], b["mean"], b["rstd"], b["x"], b["gamma"], b["beta"], M, D, 1e-5, F32)
+    ok |= lib.thvm_cuda_linear(b["h"], b["z"], b["n"], b["w1"], b["b1"], 0, M, D, H, GELU, F32)
+    ok |= lib.thvm_cuda_linear(b["y"], 0, b["h"], b["w2"], 0, b["x"], M, H, D, NONE, F32)
+    ok |= lib.thvm_cuda_linear_backward(b["dh"], b["dw2"], 0, b["dy"], 0, b["h"], b["w2"], M, H, D, NONE, F32)
+    ok |= lib.thvm_cuda_linear_backward(b["dn"], b["dw1"], b["db1"], b["dh"], b["z"], b["n"], b["w1"], M, D, H, GELU, F32)
+    ok |= lib.thvm_cuda_layernorm_backward(b["dx"], b["dgamma"], b["dbeta"], b["dn"], b["x"], b["gamma"], b["mean"], b["rstd"], M, D, F32)
+    ok |= lib.thvm_cuda_muon_step(b["w1"], b["dw1"], b["m1"], D, H, lr, 0.9, 0.01, 1, 5)
+    ok |= lib.thvm_cuda_muon_step(b["w2"], b["dw2"], b["m2"], H, D, lr, 0.9, 0.01, 1, 5)
+    assert ok == 0
+
+
+def layer_buffers(host, dims, seed):
+    M, D, H = dims
+    rng = np.random.default_rng(seed)
+    data = {"x": rng.standard_normal((M, D)), "gamma": 1 + 0.1 * rng.standard_normal(D), "beta": 0.1 * rng.standard_normal(D), "w1": spread(rng, D, H), "b1": 0.1 * rng.standard_normal(H),
+            "w2": spread(rng, H, D), "dy": 0.1 * rng.standard_normal((M, D)), "m1": np.zeros((D, H)), "m2": np.zeros((H, D))}
+    data = {k: v.astype(np.float32) for k, v in data.items()}
+    b = {k: host.up(v) for k, v in data.items()}
+    for k, n in (("n", M * D), ("mean", M), ("rstd", M), ("h", M * H), ("z", M * H), ("y", M * D), ("dh", M * H), ("dw2", H * D), ("dn", M * D), ("dw1", D * H), ("db1", H), ("dx", M * D), ("dgamma", D), ("dbeta", D)):
+        b[k] = host.out(n)
+    return data, b
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dims", [(48, 40, 96), (300, 264, 776)])
+def test_a_block_trains(host, dims):
+    """A normalised block's step, each result against the definitions fed with the results before it, and the whole gradient of x against a
+    difference of the loss sum(y dy)."""
+    M, D, H = dims
+    data, b = layer_buffers(host, dims, 5)
+    layer_step(host.lib, b, dims, 0.02)
+    f = {k: v.astype(np.float64) for k, v in data.items()}
+
+    def forward(x):
+        n, mean, rstd = norm_forward(x, f["gamma"], f["beta"], 1e-5)
+        z = n @ f["w1"] + f["b1"]
+        return act(GELU, z) @ f["w2"] + x, n, z, mean, rstd
+    y, n, z, mean, rstd = forward(f["x"])
+    dh = f["dy"] @ f["w2"].T
+    dz = dh * slope(GELU, z)
+    dn = dz @ f["w1"].T
+    dx, dgamma, dbeta = norm_backward(dn, f["x"], f["gamma"], mean, rstd)
+    got = {k: host.get(b[k], v.shape) for k, v in (("y", y), ("z", z), ("dh", dh), ("dn", dn), ("dx", dx), ("dgamma", dgamma), ("dbeta", dbeta), ("db1", dz.sum(0)), ("dw1", n.T @ dz), ("dw2", act(GELU, z).T @ f["dy"]))}
+    for k, want in (("y", y), ("z", z), ("dh", dh), ("dn", dn), ("dx", dx), ("dgamma", dgamma), ("dbeta", dbeta), ("db1", dz.sum(0)), ("dw1", n.T @ dz), ("dw2", act(GELU, z).T @ f["dy"])):
+        assert norm2(got[k], want) <= 1e-5, k                         # five stages of 2e-6 each
+    for name, dw in (("w1", n.T @ dz), ("w2", act(GELU, z).T @ f["dy"])):
+        rows, cols = dw.shape
+        want = f[name] * (1 - 0.02 * 0.01) - 0.02 * math.sqrt(max(1, rows / cols)) * newton_schulz(1.9 * dw, 5)
+        assert norm2(host.get(b[name], dw.shape), want) <= 1e-4       # the gradient's error, grown in its small directions, times the step's share
+    rng = np.random.default_rng(1)
+    v, h = rng.standard_normal((M, D)), 1e-5
+    numeric = ((forward(f["x"] + h * v)[0] - forward(f["x"] - h * v)[0]) * f["dy"]).sum() / (2 * h)
+    assert abs(numeric - ((got["dx"] + f["dy"]) * v).sum()) <= 1e-5 * np.linalg.norm(got["dx"] + f["dy"]) * np.linalg.norm(v)
+    host.done()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dims", [(48, 40, 96), (300, 264, 776)])
+def test_a_captured_block_steps_as_an_eager_one(host, dims):
+    """The step recorded once and launched twice equals two eager steps, bit for bit; a second recorded step shares the library's scratch with it;
+    and scratch that grows afterwards leaves both as they were."""
+    lib, be = host.lib, host.be
+    data, eager = layer_buffers(host, dims, 7)
+    _, rec = layer_buffers(host, dims, 7)
+    _, other = layer_buffers(host, dims, 8)
+    keep = other["dbeta"]
+    for _ in range(3):
+        layer_step(lib, eager, dims, 0.02)
+    layer_step(lib, rec, dims, 0.02)                  # the eager run that a capture needs
+    layer_step(lib, other, dims, 0.02)
+    be.reset(keep)                                    # a step's end: nothing was allocated in it
+    graphs = []
+    for b in (rec, other):
+        assert lib.thvm_cuda_capture_begin() == 0
+        layer_step(lib, b, dims, 0.02)
+        graphs.append(lib.thvm_cuda_capture_end())
+        assert graphs[-1] > 0, be.last_error()
+    assert lib.thvm_cuda_graph_launch(graphs[0]) == 0 and lib.thvm_cuda_graph_launch(graphs[1]) == 0
+    # a much larger call makes the scratch grow under the recorded steps
+    big = [host.out(n) for n in (2500 * 1100, 1100 * 1300, 2500 * 1300)]
+    assert lib.thvm_cuda_linear(big[2], 0, big[0], big[1], 0, 0, 2500, 1100, 1300, RELU, F32) == 0
+    assert lib.thvm_cuda_graph_launch(graphs[0]) == 0 and lib.thvm_cuda_graph_launch(graphs[1]) == 0
+    M, D, H = dims
+    for k, n in (("w1", D * H), ("w2", H * D), ("m1", D * H), ("y", M * D), ("dx", M * D), ("dgamma", D)):
+        assert np.array_equal(host.get(rec[k], n), host.get(eager[k], n)), k
+    for gr in graphs:
+        lib.thvm_cuda_graph_destroy(gr)
+    host.done()
+
+
+@pytest.mark.gpu
+def test_a_capture_that_would_grow_scratch_is_refused(host):
+    """Nothing runs, nothing is left over, and the same step works once it has run eagerly."""
+    lib, be = host.lib, host.be
+    M, K, N = 3000, 1500, 2100                        # its scratch is larger than that of any other test here
+    x, w, y = host.out(M * K), host.out(K * N), host.out(M * N)
+    assert lib.thvm_cuda_capture_begin() == 0
+    rc = lib.thvm_cuda_linear(y, 0, x, w, 0, 0, M, K, N, NONE, F32)
+    graph = lib.thvm_cuda_capture_end()
+    if rc == 0:                                       # (scratch was there already, from another test file)
+        assert graph > 0
+        lib.thvm_cuda_graph_destroy(graph)
+        host.done()
+        return
+    assert rc == 1 and graph == 0 and b"scratch" in last_error(lib)
+    assert lib.thvm_cuda_linear(y, 0, x, w, 0, 0, M, K, N, NONE, F32) == 0
+    assert lib.thvm_cuda_capture_begin() == 0
+    assert lib.thvm_cuda_linear(y, 0, x, w, 0, 0, M, K, N, NONE, F32) == 0
+    graph = lib.thvm_cuda_capture_end()
+    assert graph > 0 and lib.thvm_cuda_graph_launch(graph) == 0
+    assert np.all(host.get(y, M * N) == 0)
+    lib.thvm_cuda_graph_destroy(graph)
+    host.done()
+
+
+@pytest.mark.gpu
+def test_values_behind_the_last_row_stay(host):
+    """Buffers may be larger than the shape: what lies behind is neither read into the results nor written."""
+    rng = np.random.default_rng(2)
+    for M, K, N in ((3, 40, 36), (70, 64, 40), (300, 600, 700)):
+        pad = 1000
+        x, w = np.full(M * K + pad, np.nan, np.float32), np.full(K * N + pad, np.nan, np.float32)
+        x[:M * K], w[:K * N] = rng.standard_normal(M * K), rng.standard_normal(K * N)
+        y = np.full(M * max(K, N) + pad, 7.0, np.float32)
+        by, bx, bw = host.up(y), host.up(x), host.up(w)
+        assert host.lib.thvm_cuda_linear(by, 0, bx, bw, 0, 0, M, K, N, NONE, F32) == 0
+        got = host.get(by, y.size)
+        assert np.all(np.isfinite(got[:M * N])) and np.all(got[M * N:] == 7.0)
+        by = host.up(y)
+        assert host.lib.thvm_cuda_layernorm(by, 0, 0, bx, 0, 0, M, K, 1e-5, F32) == 0
+        got = host.get(by, y.size)
+        assert np.all(np.isfinite(got[:M * K])) and np.all(got[M * K:] == 7.0)
+        by = host.up(y)
+        assert host.lib.thvm_cuda_newton_schulz(by, bx, M, K, 5) == 0
+        got = host.get(by, y.size)
+        assert np.all(np.isfinite(got[:M * K])) and np.all(got[M * K:] == 7.0)
+    host.done()
+
+
+@pytest.mark.gpu
+def test_calls_among_dispatches(host):
+    """Between ordinary dispatches, which are not dependent launches: each sees what the one before wrote."""
+    lib, be = host.lib, host.be
+    M, K, N = 64, 96, 80
+    rng = np.random.default_rng(6)
+    x, w = rng.standard_normal((M, K)).astype(np.float32), rng.standard_normal((K, N)).astype(np.float32)
+    bx, bw, bt, by, bu = host.up(x), host.up(w), host.out(M * K), host.out(M * N), host.out(M * N)
+    vx, vy = abi.view_contiguous([M, K]), abi.view_contiguous([M, N])
+    for _ in range(20):
+        lib.thvm_cuda_op_unary(abi.NEG, bt, C.byref(vx), F32, bx, C.byref(vx), F32)
+        assert lib.thvm_cuda_linear(by, 0, bt, bw, 0, 0, M, K, N, RELU, F32) == 0
+        lib.thvm_cuda_op_unary(abi.NEG, bu, C.byref(vy), F32, by, C.byref(vy), F32)
+    want = -np.maximum(-(x.astype(np.float64) @ w), 0)
+    S = np.abs(x).astype(np.float64) @ np.abs(w)
+    near(host.get(bu, (M, N)), want, product_slack(K, S))
     host.done()

@@ -213,6 +213,8 @@ void capture_shutdown() {
     graphs.clear();
 }
 
+bool any_graph() { for (Capture *c : graphs) if (c) return true; return false; }
+
 static Capture *graph_of(int handle, const char *who) {
     if (handle < 1 || (size_t)handle > graphs.size() || !graphs[handle - 1]) { set_error("%s: no graph %d", who, handle); return nullptr; }
     return graphs[handle - 1];
@@ -437,6 +439,7 @@ void thvm_cuda_graph_destroy(int graph) {
     if (g.ready) cudaStreamSynchronize(g.stream);
     destroy(graphs[graph - 1]);
     graphs[graph - 1] = nullptr;
+    if (g.ready && !any_graph()) scratch_retired_free();
 }
 
 }  // extern "C"

@@ -26,7 +26,6 @@
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <string.h>
-#include <unordered_map>
 #include "layer_common.cuh"
 #include "layer_host.h"
 #include "state.h"
@@ -581,8 +580,9 @@ static Plan plan(uint32_t M, uint32_t N, uint32_t K, bool planes, bool upper) {
 
 template <uint32_t NT, class Epi>
 static void launch(const Shape &S, const Maps &maps, const Epi &epi, const char *name) {
-    static bool ready = false;
-    if (!ready) { THC_CUDA_OK(cudaFuncSetAttribute(k_hgemm<NT, Epi>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM)); ready = true; }
+    static int seen = -1;
+    if (first_on_device(seen)) THC_CUDA_OK(cudaFuncSetAttribute(k_hgemm<NT, Epi>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
+    layer_estimate(2.0 * S.M * S.N * S.K, (S.M + (double)S.N) * S.K * (S.a_lo | S.b_lo ? 4 : 2) + 4.0 * S.M * S.N);
     const uint32_t pairs = (uint32_t)g.sm_count / 2;
     profile_begin();
     chain(k_hgemm<NT, Epi>, dim3(2 * (S.tiles < pairs ? S.tiles : pairs)), THREADS, SMEM, S, maps, epi);

@@ -11,6 +11,16 @@ namespace thc {
 bool layer_buffers(const char *who, const uint32_t *ins, const uint64_t *in_need, int n_in, int in_required,
                    const uint32_t *outs, const uint64_t *out_need, int n_out, int out_required, uint32_t inplace);
 
+// Scratch of an operator, or null where a captured step would need more than there is (the reason is in the sticky error; the capture
+// is refused at its end).
+void *layer_scratch(const char *who, uint64_t bytes);
+
+// Whether this is the first call for the current device with this `seen` (-1 at first): kernel attributes belong to a device.
+static inline bool first_on_device(int &seen) { if (seen == g.device) return false; seen = g.device; return true; }
+
+// what profile_report says of the launch that comes next
+static inline void layer_estimate(double ops, double bytes) { if (g.profile) { g.prof_ops = (unsigned long long)ops; g.prof_bytes = (unsigned long long)bytes; } }
+
 // Launches a kernel that begins with depend() (layer_common.cuh) on the backend's stream.  The set-up of a kernel and its blocks' start
 // overlap the end of the kernel before it, which is worth some 2 us of the 4 that a launch in a chain costs.
 // cluster_y: blocks of a cluster along y, where the kernel does not say itself.

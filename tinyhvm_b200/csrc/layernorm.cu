@@ -317,7 +317,7 @@ static void norm_bwd_launch_g(uint32_t group, void *dx, float *partial, const vo
     }
 }
 template <typename T>
-static void norm_backward(void *dx, void *dgamma, void *dbeta, const void *dy, const void *x, const void *gamma, const float *mean, const float *rstd, uint32_t rows, uint32_t cols) {
+static bool norm_backward(void *dx, void *dgamma, void *dbeta, const void *dy, const void *x, const void *gamma, const float *mean, const float *rstd, uint32_t rows, uint32_t cols) {
     const uint32_t group = norm_group(cols, NORM_BWD_VALUES);
     const bool sums = dgamma || dbeta;
     uint32_t n;
@@ -327,14 +327,14 @@ static void norm_backward(void *dx, void *dgamma, void *dbeta, const void *dy, c
         const uint32_t threads = group > 32 ? group : NORM_BLOCK, per = group > 32 ? 1 : NORM_BLOCK / 32;
         // 1024 threads an SM: the registers allow no more; and four rows a group at least, for the sums' sake
         n = grid_for((rows + 3) / 4, per, 1024 / threads);
-        if (sums) partial = (float *)scratch_reserve((uint64_t)n * 2 * cols * sizeof(float));
+        if (sums && !(partial = (float *)layer_scratch("layernorm_backward", (uint64_t)n * 2 * cols * sizeof(float)))) return false;
         if (cols % Vec16<T>::n == 0) norm_bwd_launch_g<T, Vec16<T>::n>(group, dx, partial, dy, x, gamma, mean, rstd, rows, cols, n);
         else norm_bwd_launch_g<T, 1>(group, dx, partial, dy, x, gamma, mean, rstd, rows, cols, n);
         after_launch("layernorm_backward");
     } else {
         n = rows < 16 ? rows : 16;
         if (sums) {                                    // first: dx may lie where dy or x does
-            partial = (float *)scratch_reserve((uint64_t)n * 2 * cols * sizeof(float));
+            if (!(partial = (float *)layer_scratch("layernorm_backward", (uint64_t)n * 2 * cols * sizeof(float)))) return false;
             chain(k_norm_bwd_cols<T>, dim3((cols + 255) / 256, n), 256, 0, partial, (const T *)dy, (const T *)x, mean, rstd, rows, cols);
             after_launch("layernorm_backward_cols");
             profile_begin();
@@ -349,6 +349,7 @@ static void norm_backward(void *dx, void *dgamma, void *dbeta, const void *dy, c
         chain(k_fold_rows<T>, dim3((cols + 31) / 32, 2), 1024, 0, (T *)dgamma, (T *)dbeta, (const float *)partial, n, cols);
         after_launch("layernorm_fold");
     }
+    return true;
 }
 
 }  // namespace thc
@@ -360,6 +361,7 @@ extern "C" {
 int thvm_cuda_layernorm(uint32_t y, uint32_t mean, uint32_t rstd, uint32_t x, uint32_t gamma, uint32_t beta,
                         uint32_t rows, uint32_t cols, float eps, uint32_t dtype) {
     if (rows == 0 || cols == 0) { set_error("layernorm: empty shape"); return 1; }
+    if (rows > (1u << 30) || cols > (1u << 30)) { set_error("layernorm: a dimension exceeds 2^30"); return 1; }
     if (dtype != THC_F32 && dtype != THC_F16) { set_error("layernorm: dtype %u is neither f32 nor f16", dtype); return 1; }
     if (!(eps >= 0.0f)) { set_error("layernorm: eps %g", (double)eps); return 1; }
     const uint64_t sz = dtype == THC_F16 ? 2 : 4, need = (uint64_t)rows * cols * sz;
@@ -372,6 +374,7 @@ int thvm_cuda_layernorm(uint32_t y, uint32_t mean, uint32_t rstd, uint32_t x, ui
     float *pm = mean ? (float *)buf_for_output(mean, "layernorm(mean)", (uint64_t)rows * 4).ptr : nullptr;
     float *pr = rstd ? (float *)buf_for_output(rstd, "layernorm(rstd)", (uint64_t)rows * 4).ptr : nullptr;
     for (uint32_t id : outs) if (id) mark_device_written(id);
+    layer_estimate(8.0 * rows * cols, 2.0 * need);
     profile_begin();
     if (dtype == THC_F16) norm_forward<__half>(py, pm, pr, px, pg, pb, rows, cols, eps);
     else norm_forward<float>(py, pm, pr, px, pg, pb, rows, cols, eps);
@@ -382,6 +385,7 @@ int thvm_cuda_layernorm(uint32_t y, uint32_t mean, uint32_t rstd, uint32_t x, ui
 int thvm_cuda_layernorm_backward(uint32_t dx, uint32_t dgamma, uint32_t dbeta, uint32_t dy, uint32_t x, uint32_t gamma,
                                  uint32_t mean, uint32_t rstd, uint32_t rows, uint32_t cols, uint32_t dtype) {
     if (rows == 0 || cols == 0) { set_error("layernorm_backward: empty shape"); return 1; }
+    if (rows > (1u << 30) || cols > (1u << 30)) { set_error("layernorm_backward: a dimension exceeds 2^30"); return 1; }
     if (dtype != THC_F32 && dtype != THC_F16) { set_error("layernorm_backward: dtype %u is neither f32 nor f16", dtype); return 1; }
     if (!dx && !dgamma && !dbeta) { set_error("layernorm_backward: no output asked for"); return 1; }
     const uint64_t sz = dtype == THC_F16 ? 2 : 4, need = (uint64_t)rows * cols * sz;
@@ -395,9 +399,8 @@ int thvm_cuda_layernorm_backward(uint32_t dx, uint32_t dgamma, uint32_t dbeta, u
     void *pdg = dgamma ? buf_for_output(dgamma, "layernorm_backward(dgamma)", cols * sz).ptr : nullptr;
     void *pdb = dbeta ? buf_for_output(dbeta, "layernorm_backward(dbeta)", cols * sz).ptr : nullptr;
     for (uint32_t id : outs) if (id) mark_device_written(id);
-    if (dtype == THC_F16) norm_backward<__half>(pdx, pdg, pdb, pdy, px, pg, pm, pr, rows, cols);
-    else norm_backward<float>(pdx, pdg, pdb, pdy, px, pg, pm, pr, rows, cols);
-    return 0;
+    layer_estimate(14.0 * rows * cols, 3.0 * need);
+    return (dtype == THC_F16 ? norm_backward<__half>(pdx, pdg, pdb, pdy, px, pg, pm, pr, rows, cols) : norm_backward<float>(pdx, pdg, pdb, pdy, px, pg, pm, pr, rows, cols)) ? 0 : 1;
 }
 
 }  // extern "C"

@@ -10,6 +10,12 @@
 
 namespace thc {
 
+void *layer_scratch(const char *who, uint64_t bytes) {
+    void *p = scratch_reserve(bytes);
+    if (scratch_short(bytes)) { set_error("%s: library scratch had to grow inside the captured step: run the step once before capturing it", who); return nullptr; }
+    return p;
+}
+
 bool layer_buffers(const char *who, const uint32_t *ins, const uint64_t *in_need, int n_in, int in_required,
                    const uint32_t *outs, const uint64_t *out_need, int n_out, int out_required, uint32_t inplace) {
     for (int side = 0; side < 2; side++) {
@@ -444,8 +450,9 @@ static hg::Operand f16_operand(Cut &c, const __half *p, uint32_t rows, uint32_t 
 
 template <typename T, int MR, int V>
 static void few_rows_as(void *y, void *z, const void *x, const void *w, const void *bias, const void *residual, uint32_t M, uint32_t K, uint32_t N, uint32_t act) {
-    static bool ready = false;
-    if (!ready) { THC_CUDA_OK(cudaFuncSetAttribute(k_linear_few<T, MR, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)few_smem<T, MR, V>())); ready = true; }
+    static int seen = -1;
+    if (first_on_device(seen)) THC_CUDA_OK(cudaFuncSetAttribute(k_linear_few<T, MR, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)few_smem<T, MR, V>()));
+    layer_estimate(2.0 * M * K * N, ((double)K * N + (double)M * K + (double)M * N) * sizeof(T));
     chain(k_linear_few<T, MR, V>, dim3((N + 32 * V - 1) / (32 * V), (M + MR - 1) / MR * FEW_CLUSTER), 256, few_smem<T, MR, V>(), (T *)y, (T *)z, (const T *)x, (const T *)w, (const T *)bias, (const T *)residual, M, K, N, act);
 }
 // Up to how many rows the kernel above is taken, from 4096 x 4096 weights.  f32: 15 us for one row, 19 for eight, 37 for 16, 53 for 24, 68 for 32;
@@ -475,18 +482,19 @@ constexpr double SMALL_FORWARD = 1e8, SMALL_BACKWARD_F32 = 4e7, SMALL_BACKWARD_F
 constexpr uint32_t SMALL_BACKWARD_ROWS = 1024;
 
 template <typename T>
-static void linear_forward(void *y, void *z, const void *x, const void *w, const void *bias, const void *residual, uint32_t M, uint32_t K, uint32_t N, uint32_t act) {
+static bool linear_forward(void *y, void *z, const void *x, const void *w, const void *bias, const void *residual, uint32_t M, uint32_t K, uint32_t N, uint32_t act) {
     constexpr bool F = sizeof(T) == 4;
-    if (few_rows<T>(y, z, x, w, bias, residual, M, K, N, act)) return;
+    if (few_rows<T>(y, z, x, w, bias, residual, M, K, N, act)) return true;
     if constexpr (F) if ((double)M * K * N <= SMALL_FORWARD) {
         Small<T> S{};
         S.x = (const T *)x; S.w = (const T *)w; S.bias = (const T *)bias; S.residual = (const T *)residual; S.y = (T *)y; S.z_out = (T *)z;
         S.M = M; S.K = K; S.N = N; S.act = act;
         const uint32_t tiles = ((M + 31) / 32) * ((N + 31) / 32), ranks = small_ranks(tiles, K, 8);
+        layer_estimate(2.0 * M * K * N, ((double)K * N + (double)M * K + (double)M * N) * sizeof(T));
         profile_begin();
         chain_cluster(ranks, k_small_forward<T>, dim3(tiles, ranks), 128, 0, S);
         after_launch("linear_small");
-        return;
+        return true;
     }
     const hg::Plan plan = hg::plan(M, N, K, F, false);
     const int *exps = nullptr;
@@ -494,7 +502,11 @@ static void linear_forward(void *y, void *z, const void *x, const void *w, const
     hg::Operand A{}, B{};
     float *partial = nullptr;
     for (int pass = 0; pass < 2; pass++) {             // the first pass measures
-        if (pass) { c.base = (uint8_t *)scratch_reserve(c.at); c.at = 0; }
+        if (pass) {
+            c.base = (uint8_t *)layer_scratch("linear", c.at);
+            if (!c.base && c.at) return false;
+            c.at = 0;
+        }
         partial = c.take<float>(plan.partial_bytes / 4);
         if constexpr (F) {
             const Planes pw = take_planes(c, K, N, true, true, K), px = take_planes(c, M, K, true, true, M);
@@ -518,10 +530,11 @@ static void linear_forward(void *y, void *z, const void *x, const void *w, const
         case THC_ACT_SILU: run(LayerEpi<T, THC_ACT_SILU>{ty, tz, tb, tr, exps, N, {}}); break;
         default:           run(LayerEpi<T, THC_ACT_NONE>{ty, tz, tb, tr, exps, N, {}}); break;
     }
+    return true;
 }
 
 template <typename T>
-static void linear_backward(void *dx, void *dw, void *dbias, const void *dy, const void *z, const void *x, const void *w, uint32_t M, uint32_t K, uint32_t N, uint32_t act) {
+static bool linear_backward(void *dx, void *dw, void *dbias, const void *dy, const void *z, const void *x, const void *w, uint32_t M, uint32_t K, uint32_t N, uint32_t act) {
     constexpr bool F = sizeof(T) == 4;
     if ((double)M * K * N <= (F ? SMALL_BACKWARD_F32 : SMALL_BACKWARD_F16) && M <= SMALL_BACKWARD_ROWS) {
         Small<T> S{};
@@ -530,10 +543,11 @@ static void linear_backward(void *dx, void *dw, void *dbias, const void *dy, con
         const uint32_t m = (M + 31) / 32, k = (K + 31) / 32, n = (N + 31) / 32, ranks = small_ranks((uint64_t)m * k + k * n, M > N ? M : N, 16);   // (whatever is asked for)
         S.dx_tiles = dx ? m * k : 0;
         const uint32_t tiles = S.dx_tiles + (dw ? k * n : dbias ? n : 0);      // the bias's gradient comes from dw's first row of tiles
+        layer_estimate(4.0 * M * K * N, 2.0 * ((double)K * N + (double)M * K + (double)M * N) * sizeof(T));
         profile_begin();
         chain_cluster(ranks, k_small_backward<T>, dim3(tiles, ranks), 128, 0, S);
         after_launch("linear_backward_small");
-        return;
+        return true;
     }
     const bool smooth = act == THC_ACT_GELU || act == THC_ACT_SILU;
     const bool scaled = F || smooth;                   // dz needs planes: f32, or f16 times a slope that is neither 0 nor 1
@@ -543,7 +557,11 @@ static void linear_backward(void *dx, void *dw, void *dbias, const void *dy, con
     const uint32_t blocks = dbias ? grid_for(M, 1, 4) : split_blocks(M), sum_rows = N > ROW_VALUES ? (M < 16 ? M : 16) : blocks;
     Cut c;
     for (int pass = 0; pass < 2; pass++) {
-        if (pass) { c.base = (uint8_t *)scratch_reserve(c.at); c.at = 0; }
+        if (pass) {
+            c.base = (uint8_t *)layer_scratch("linear_backward", c.at);
+            if (!c.base && c.at) return false;
+            c.at = 0;
+        }
         float *partial = c.take<float>((plan_x.partial_bytes > plan_w.partial_bytes ? plan_x.partial_bytes : plan_w.partial_bytes) / 4);
         // dz, and its sums over rows
         Planes pz{};
@@ -595,6 +613,7 @@ static void linear_backward(void *dx, void *dw, void *dbias, const void *dy, con
             if (pass) hg::product(X, dz_mn, K, N, M, plan_w, partial, GradEpi<T, false>{(T *)dw, exps, nullptr, N, {}}, false, "linear_backward_dw");
         }
     }
+    return true;
 }
 
 static bool linear_shape(const char *who, uint32_t M, uint32_t K, uint32_t N, uint32_t act, uint32_t dtype) {
@@ -623,9 +642,7 @@ int thvm_cuda_linear(uint32_t y, uint32_t z, uint32_t x, uint32_t w, uint32_t bi
     void *py = buf_for_output(y, "linear(y)", mn).ptr, *pz = z ? buf_for_output(z, "linear(z)", mn).ptr : nullptr;
     mark_device_written(y);
     if (z) mark_device_written(z);
-    if (dtype == THC_F16) linear_forward<__half>(py, pz, px, pw, pb, pr, M, K, N, act);
-    else linear_forward<float>(py, pz, px, pw, pb, pr, M, K, N, act);
-    return 0;
+    return (dtype == THC_F16 ? linear_forward<__half>(py, pz, px, pw, pb, pr, M, K, N, act) : linear_forward<float>(py, pz, px, pw, pb, pr, M, K, N, act)) ? 0 : 1;
 }
 
 int thvm_cuda_linear_backward(uint32_t dx, uint32_t dw, uint32_t dbias, uint32_t dy, uint32_t z, uint32_t x, uint32_t w,
@@ -646,9 +663,7 @@ int thvm_cuda_linear_backward(uint32_t dx, uint32_t dw, uint32_t dbias, uint32_t
     void *pdw = dw ? buf_for_output(dw, "linear_backward(dw)", kn).ptr : nullptr;
     void *pdb = dbias ? buf_for_output(dbias, "linear_backward(dbias)", N * sz).ptr : nullptr;
     for (uint32_t id : outs) if (id) mark_device_written(id);
-    if (dtype == THC_F16) linear_backward<__half>(pdx, pdw, pdb, pdy, pz, px, pw, M, K, N, act);
-    else linear_backward<float>(pdx, pdw, pdb, pdy, pz, px, pw, M, K, N, act);
-    return 0;
+    return (dtype == THC_F16 ? linear_backward<__half>(pdx, pdw, pdb, pdy, pz, px, pw, M, K, N, act) : linear_backward<float>(pdx, pdw, pdb, pdy, pz, px, pw, M, K, N, act)) ? 0 : 1;
 }
 
 }  // extern "C"

@@ -289,8 +289,8 @@ k_ns_small(const __grid_constant__ NsSmall S) {
 // the cluster's size for a matrix, or 0 where it does not fit; 16 blocks need the GPU's consent
 static uint32_t ns_small_ranks(uint32_t m, uint32_t n) {
     if (m > NS_SIDE || n > NS_SHARE * 16) return 0;
-    static int most = 0;
-    if (!most) {
+    static int most = 0, seen = -1;
+    if (first_on_device(seen)) {
         most = 8;
         THC_CUDA_OK(cudaFuncSetAttribute(k_ns_small, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)NS_SMEM));
         THC_CUDA_OK(cudaFuncSetAttribute(k_ns_small, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
@@ -307,22 +307,24 @@ static uint32_t ns_small_ranks(uint32_t m, uint32_t n) {
 }
 
 // out (or the parameter step, when param is given) <- Newton-Schulz of grad or of the momentum update
-static void newton_schulz(float *out, float *param, float *mom, const float *grad, uint32_t rows, uint32_t cols, uint32_t steps, float mu, int nesterov, float keep, float step) {
+static bool newton_schulz(float *out, float *param, float *mom, const float *grad, uint32_t rows, uint32_t cols, uint32_t steps, float mu, int nesterov, float keep, float step) {
     const uint64_t n = (uint64_t)rows * cols;
     const bool wide = rows <= cols;
     const uint32_t m = wide ? rows : cols, k = wide ? cols : rows;
     if (const uint32_t ranks = ns_small_ranks(m, k)) {
+        layer_estimate(2.0 * steps * m * m * (2.0 * k + m), 4.0 * rows * cols * (param ? 5 : 2));
         profile_begin();
         chain_cluster(ranks, k_ns_small, dim3(1, ranks), 256, NS_SMEM, NsSmall{out, param, mom, grad, rows, cols, steps, nesterov, mu, keep, step});
         after_launch("newton_schulz_small");
-        return;
+        return true;
     }
     const uint64_t px = (cols + 63u) & ~63ull, pm = (m + 63u) & ~63ull, x_bytes = rows * px * 2, m_bytes = m * pm * 2;    // (multiples of 128)
     const unsigned blocks = grid_for(n, 1024, 4);
     const hg::Plan square = hg::plan(m, m, k, true, true), poly = hg::plan(m, m, m, true, true), apply = hg::plan(rows, cols, m, true, false);
     uint64_t partial_bytes = square.partial_bytes > poly.partial_bytes ? square.partial_bytes : poly.partial_bytes;
     if (apply.partial_bytes > partial_bytes) partial_bytes = apply.partial_bytes;
-    uint8_t *base = (uint8_t *)scratch_reserve(4 * x_bytes + 4 * m_bytes + ((partial_bytes + 7) & ~7ull) + blocks * sizeof(double));
+    uint8_t *base = (uint8_t *)layer_scratch(mom ? "muon_step" : "newton_schulz", 4 * x_bytes + 4 * m_bytes + ((partial_bytes + 7) & ~7ull) + blocks * sizeof(double));
+    if (!base) return false;
     __half *x[2][2], *a[2], *b[2];
     for (int i = 0; i < 2; i++) {
         for (int p = 0; p < 2; p++) x[i][p] = (__half *)(base + (2 * i + p) * x_bytes);
@@ -350,6 +352,7 @@ static void newton_schulz(float *out, float *param, float *mom, const float *gra
         else if (param) run(ApplyEpi<STEP>{nullptr, nullptr, 0, param, cols, keep, step});
         else run(ApplyEpi<RESULT>{nullptr, nullptr, 0, out, cols, 0.0f, 0.0f});
     }
+    return true;
 }
 
 static bool ns_shape(const char *who, uint32_t rows, uint32_t cols, uint32_t steps) {
@@ -372,8 +375,7 @@ int thvm_cuda_newton_schulz(uint32_t out, uint32_t x, uint32_t rows, uint32_t co
     const float *px = (const float *)buf_checked(x, "newton_schulz(x)").ptr;
     float *po = (float *)buf_for_output(out, "newton_schulz(out)", need).ptr;
     mark_device_written(out);
-    newton_schulz(po, nullptr, nullptr, px, rows, cols, steps, 0.0f, 0, 0.0f, 0.0f);
-    return 0;
+    return newton_schulz(po, nullptr, nullptr, px, rows, cols, steps, 0.0f, 0, 0.0f, 0.0f) ? 0 : 1;
 }
 
 int thvm_cuda_muon_step(uint32_t param, uint32_t grad, uint32_t momentum, uint32_t rows, uint32_t cols,
@@ -386,8 +388,7 @@ int thvm_cuda_muon_step(uint32_t param, uint32_t grad, uint32_t momentum, uint32
     float *pp = (float *)buf_checked(param, "muon_step(param)").ptr, *pm = (float *)buf_checked(momentum, "muon_step(momentum)").ptr;
     mark_device_written(param); mark_device_written(momentum);
     const double ratio = (double)rows / (double)cols;
-    newton_schulz(nullptr, pp, pm, pg, rows, cols, steps, mu, nesterov != 0, (float)(1.0 - (double)lr * weight_decay), (float)((double)lr * sqrt(ratio > 1.0 ? ratio : 1.0)));
-    return 0;
+    return newton_schulz(nullptr, pp, pm, pg, rows, cols, steps, mu, nesterov != 0, (float)(1.0 - (double)lr * weight_decay), (float)((double)lr * sqrt(ratio > 1.0 ? ratio : 1.0))) ? 0 : 1;
 }
 
 }  // extern "C"

@@ -23,6 +23,7 @@
 #include <stdarg.h>
 #include <string.h>
 #include <map>
+#include <vector>
 #include "state.h"
 
 namespace thc {
@@ -131,10 +132,19 @@ Buf &buf_for_output(uint32_t id, const char *who, uint64_t bytes_written) {
     return r;
 }
 
+static std::vector<void *> &retired() { static std::vector<void *> *v = new std::vector<void *>(); return *v; }
+void scratch_retired_free() {
+    for (void *p : retired()) cudaFreeAsync(p, g.stream);
+    retired().clear();
+}
+bool scratch_short(uint64_t bytes) { return bytes > g.scratch_bytes; }
+
 void *scratch_reserve(uint64_t bytes) {
     if (bytes <= g.scratch_bytes) return g.scratch;
     if (g.cap) { capture_fail("library scratch had to grow inside the captured step: run the step once before capturing it"); return g.scratch; }
-    if (g.scratch) THC_CUDA_OK(cudaFreeAsync(g.scratch, g.stream));
+    // a recorded step goes on using the scratch that it was recorded with: kept until the last of them is destroyed
+    if (g.scratch && any_graph()) retired().push_back(g.scratch);
+    else if (g.scratch) THC_CUDA_OK(cudaFreeAsync(g.scratch, g.stream));
     uint64_t want = bytes + (bytes >> 2);
     THC_CUDA_OK(cudaMallocAsync(&g.scratch, want, g.stream));
     g.scratch_bytes = want;
@@ -299,6 +309,7 @@ void thvm_cuda_shutdown(void) {
     for (uint32_t i = 1; i < g.count; i++) if (g.bufs[i].live) release(i);
     plan_cache_clear();
     if (g.scratch) cudaFreeAsync(g.scratch, g.stream);
+    scratch_retired_free();
     g.scratch = nullptr; g.scratch_bytes = 0;
     cudaStreamSynchronize(g.stream);
     cudaFree(g.dev_status); g.dev_status = nullptr;

@@ -88,8 +88,11 @@ Buf &buf_checked(uint32_t id, const char *who);
 Buf &buf_for_output(uint32_t id, const char *who, uint64_t bytes_written);
 // a live buffer that may still be host-only
 Buf &buf_live(uint32_t id, const char *who);
-// scratch of at least `bytes` (stream-ordered reuse: all users run on g.stream)
+// scratch of at least `bytes` (stream-ordered reuse: all users run on g.stream).  While a step is being captured it does not grow: the
+// capture is marked unusable and what there is (less than `bytes`, perhaps null) comes back; callers that put addresses of it into
+// anything that is checked test scratch_short(bytes) first.
 void *scratch_reserve(uint64_t bytes);
+bool scratch_short(uint64_t bytes);
 // before `b` is overwritten or freed on the main stream: wait for a read-back of it that may still be running
 void fence_copy(Buf &b);
 // mark a buffer as written by the device
@@ -125,5 +128,7 @@ uint8_t *capture_arena_take(uint64_t bytes);                    // pinned host m
 int  capture_add_input(void *dst, const void *src, uint64_t bytes);
 void capture_add_result(const void *src, uint64_t bytes);
 void capture_shutdown();
+bool any_graph();                                               // whether a recorded step is alive (it may hold addresses of library scratch)
+void scratch_retired_free();                                    // pool.cu: scratch that was replaced while recorded steps held it
 
 }  // namespace thc
