@@ -489,7 +489,7 @@ static bool linear_forward(void *y, void *z, const void *x, const void *w, const
         Small<T> S{};
         S.x = (const T *)x; S.w = (const T *)w; S.bias = (const T *)bias; S.residual = (const T *)residual; S.y = (T *)y; S.z_out = (T *)z;
         S.M = M; S.K = K; S.N = N; S.act = act;
-        const uint32_t tiles = ((M + 31) / 32) * ((N + 31) / 32), ranks = small_ranks(tiles, K, 8);
+        const uint32_t tiles = ((M + SMALL_ROWS - 1) / SMALL_ROWS) * ((N + 31) / 32), ranks = small_ranks(tiles, K, 8);
         layer_estimate(2.0 * M * K * N, ((double)K * N + (double)M * K + (double)M * N) * sizeof(T));
         profile_begin();
         chain_cluster(ranks, k_small_forward<T>, dim3(tiles, ranks), 128, 0, S);
@@ -540,8 +540,9 @@ static bool linear_backward(void *dx, void *dw, void *dbias, const void *dy, con
         Small<T> S{};
         S.x = (const T *)x; S.w = (const T *)w; S.dy = (const T *)dy; S.z_in = (const T *)z; S.dx = (T *)dx; S.dw = (T *)dw; S.dbias = (T *)dbias;
         S.M = M; S.K = K; S.N = N; S.act = act;
-        const uint32_t m = (M + 31) / 32, k = (K + 31) / 32, n = (N + 31) / 32, ranks = small_ranks((uint64_t)m * k + k * n, M > N ? M : N, 16);   // (whatever is asked for)
-        S.dx_tiles = dx ? m * k : 0;
+        const uint32_t m = (M + SMALL_ROWS - 1) / SMALL_ROWS, k = (K + SMALL_ROWS - 1) / SMALL_ROWS, k32 = (K + 31) / 32, n = (N + 31) / 32;
+        const uint32_t ranks = small_ranks((uint64_t)m * k32 + k * n, M > N ? M : N, 16);                  // (whatever is asked for)
+        S.dx_tiles = dx ? m * k32 : 0;
         const uint32_t tiles = S.dx_tiles + (dw ? k * n : dbias ? n : 0);      // the bias's gradient comes from dw's first row of tiles
         layer_estimate(4.0 * M * K * N, 2.0 * ((double)K * N + (double)M * K + (double)M * N) * sizeof(T));
         profile_begin();

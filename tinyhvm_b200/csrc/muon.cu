@@ -157,10 +157,10 @@ template <int TO> struct ApplyEpi {                    // X = (a I + b A + c A A
 // The smaller side is at most 128, the larger 32 times the cluster.  Block r of the cluster keeps every row of its own share of the larger
 // side's columns, X_r (stored column by column), and A and B whole.  A step: P_r = X_r X_r^T by each block; A = sum of P_r, an equal share
 // of rows by each block, written to all; B = a I + b A + c A A the same way; X_r = B X_r.  Three barriers of the cluster a step.  All in
-// f32 on the CUDA cores: 0.03 GFLOP a step at 400 x 120 is nothing; what bounds it is the latency of the shared-memory reads with two warps a
+// f32 on the CUDA cores: 0.03 GFLOP a step at 400 x 120 is nothing; what bounds it is the latency of the shared-memory reads with four warps a
 // scheduler and of the exchange.  As 15 launches of the matrix engine the same step takes 164 us.
-constexpr uint32_t NS_SIDE = 128, NS_SHARE = 32, NS_PITCH = 132;
-constexpr size_t NS_SMEM = (size_t)(NS_SHARE + 2 * NS_SIDE) * NS_PITCH * 4;
+constexpr uint32_t NS_SIDE = 128, NS_SHARE = 32, NS_PITCH = 132, NS_THREADS = 512, NS_WARPS = NS_THREADS / 32;
+constexpr size_t NS_SMEM = (size_t)(NS_SHARE + 2 * NS_SIDE) * NS_PITCH * 4 + (size_t)NS_WARPS * 8 * NS_SIDE * 4;     // X, A, B; the warps' parts of B's rows
 struct NsSmall { float *out, *param, *mom; const float *grad; uint32_t rows, cols, steps; int nesterov; float mu, keep, step; };
 
 __device__ __forceinline__ float4 remote4(const float *p, uint32_t rank) {
@@ -171,21 +171,22 @@ __device__ __forceinline__ float4 remote4(const float *p, uint32_t rank) {
 __device__ __forceinline__ void remote4(float *p, uint32_t rank, float4 v) {
     asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(hg::in_cta(hg::smem32(p), rank)), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
-__global__ void __launch_bounds__(256, 1)
+__global__ void __launch_bounds__(NS_THREADS, 1)
 k_ns_small(const __grid_constant__ NsSmall S) {
     depend();
     extern __shared__ __align__(16) float ns[];
     float (*X)[NS_PITCH] = reinterpret_cast<float (*)[NS_PITCH]>(ns);                              // [NS_SHARE]: column, row
     float (*A)[NS_PITCH] = X + NS_SHARE, (*B)[NS_PITCH] = A + NS_SIDE;                             // [NS_SIDE]; B first holds P
-    __shared__ double red[8], norm;
-    const uint32_t ranks = gridDim.y, rank = blockIdx.y, tid = threadIdx.x;
+    float4 *parts = reinterpret_cast<float4 *>(B + NS_SIDE);                                       // [NS_WARPS][8][32]
+    __shared__ double red[NS_WARPS], norm;
+    const uint32_t ranks = gridDim.y, rank = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const bool wide = S.rows <= S.cols;
     const uint32_t m = wide ? S.rows : S.cols, n = wide ? S.cols : S.rows, share = (n + ranks - 1) / ranks;
     const uint32_t c0 = rank * share, mine = c0 >= n ? 0 : n - c0 < share ? n - c0 : share;        // columns c0 .. c0 + mine
     // the update, its place in memory and its sum of squares; rows and columns beyond the matrix are zeros
     const auto place = [&](uint32_t c, uint32_t r) { return wide ? (uint64_t)r * S.cols + c0 + c : (uint64_t)(c0 + c) * S.cols + r; };
     const auto each = [&](auto f) {                        // lanes along memory
-        for (uint32_t u = tid; u < NS_SHARE * NS_SIDE; u += 256) { const uint32_t c = wide ? u % NS_SHARE : u / NS_SIDE, r = wide ? u / NS_SHARE : u % NS_SIDE; f(c, r, c < mine && r < m); }
+        for (uint32_t u = tid; u < NS_SHARE * NS_SIDE; u += NS_THREADS) { const uint32_t c = wide ? u % NS_SHARE : u / NS_SIDE, r = wide ? u / NS_SHARE : u % NS_SIDE; f(c, r, c < mine && r < m); }
     };
     double sq = 0.0;
     each([&](uint32_t c, uint32_t r, bool in) {
@@ -202,7 +203,7 @@ k_ns_small(const __grid_constant__ NsSmall S) {
     for (int o = 16; o; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
     if ((tid & 31) == 0) red[tid >> 5] = sq;
     __syncthreads();
-    if (tid == 0) { double s = 0.0; for (int w = 0; w < 8; w++) s += red[w]; norm = s; }
+    if (tid == 0) { double s = 0.0; for (uint32_t w = 0; w < NS_WARPS; w++) s += red[w]; norm = s; }
     hg::cluster_sync();
     double total = 0.0;
     for (uint32_t q = 0; q < ranks; q++) {
@@ -215,66 +216,90 @@ k_ns_small(const __grid_constant__ NsSmall S) {
     const uint32_t band = NS_SIDE / ranks;                 // rows of A and of B that this block makes
     for (uint32_t step = 0; step < S.steps; step++) {
         __syncthreads();
-        {   // P = X_r X_r^T: 8 x 8 sums a thread
-            const uint32_t r0 = (tid >> 4) * 8, q0 = (tid & 15u) * 4;          // rows r0 .., columns q0 .. and q0 + 64 ..
-            float acc[8][8] = {};
+        {   // P = X_r X_r^T: 8 x 4 sums a thread
+            const uint32_t r0 = warp * 8, q0 = lane * 4;
+            float acc[8][4] = {};
+#pragma unroll 2
             for (uint32_t k = 0; k < mine; k++) {
-                const float4 a0 = *reinterpret_cast<const float4 *>(&X[k][r0]), a1 = *reinterpret_cast<const float4 *>(&X[k][r0 + 4]);
-                const float4 b0 = *reinterpret_cast<const float4 *>(&X[k][q0]), b1 = *reinterpret_cast<const float4 *>(&X[k][q0 + 64]);
-                const float a[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w}, b[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
+                const float4 a0 = *reinterpret_cast<const float4 *>(&X[k][r0]), a1 = *reinterpret_cast<const float4 *>(&X[k][r0 + 4]), b = *reinterpret_cast<const float4 *>(&X[k][q0]);
+                const float a[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-#pragma unroll
-                    for (int j = 0; j < 8; j++) acc[i][j] += a[i] * b[j];
+                for (int i = 0; i < 8; i++) { acc[i][0] += a[i] * b.x; acc[i][1] += a[i] * b.y; acc[i][2] += a[i] * b.z; acc[i][3] += a[i] * b.w; }
             }
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                *reinterpret_cast<float4 *>(&B[r0 + i][q0]) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
-                *reinterpret_cast<float4 *>(&B[r0 + i][q0 + 64]) = make_float4(acc[i][4], acc[i][5], acc[i][6], acc[i][7]);
-            }
+            for (int i = 0; i < 8; i++) *reinterpret_cast<float4 *>(&B[r0 + i][q0]) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
         }
         hg::cluster_sync();
-        for (uint32_t u = tid; u < band * 32; u += 256) {   // this block's rows of A, to every block
-            const uint32_t r = rank * band + u / 32, c = u % 32 * 4;
+        // this block's rows of A: the two halves of the block add the P of half of the ranks each, and write to half of them
+        for (uint32_t i0 = 0; i0 < band; i0 += 8) {
+            const uint32_t r = rank * band + i0 + (warp & 7u), c = lane * 4, side = warp >> 3, some = ranks / 2;
             float4 s = make_float4(0, 0, 0, 0);
 #pragma unroll 8
-            for (uint32_t q = 0; q < ranks; q++) { const float4 v = remote4(&B[r][c], q); s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w; }
+            for (uint32_t q = side * some; q < (side + 1) * some; q++) { const float4 v = remote4(&B[r][c], q); s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w; }
+            parts[tid] = s;
+            __syncthreads();
+            const float4 x = parts[tid & 255u], y = parts[(tid & 255u) + 256u];
+            s = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
 #pragma unroll 8
-            for (uint32_t q = 0; q < ranks; q++) remote4(&A[r][c], q, s);
+            for (uint32_t q = side * some; q < (side + 1) * some; q++) remote4(&A[r][c], q, s);
+            __syncthreads();
         }
         hg::cluster_sync();
-        for (uint32_t u = tid; u < band * 32; u += 256) {   // its rows of a I + b A + c A A
-            const uint32_t r = rank * band + u / 32, c = u % 32 * 4;
-            float4 s = make_float4(0, 0, 0, 0);
-#pragma unroll 8
-            for (uint32_t k = 0; k < NS_SIDE; k++) {
-                const float a = A[r][k];
-                const float4 b = *reinterpret_cast<const float4 *>(&A[k][c]);
-                s.x += a * b.x; s.y += a * b.y; s.z += a * b.z; s.w += a * b.w;
+        // its rows of a I + b A + c A A: a warp sums an equal share of the contraction for eight whole rows, the parts are added in warp order
+        for (uint32_t i0 = 0; i0 < band; i0 += 8) {
+            const uint32_t r0 = rank * band + i0;
+            float4 acc[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) acc[i] = make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (uint32_t k0 = 0; k0 < NS_SIDE / NS_WARPS; k0 += 4) {
+                const uint32_t k = warp * (NS_SIDE / NS_WARPS) + k0;
+                float4 b[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) b[j] = *reinterpret_cast<const float4 *>(&A[k + j][lane * 4]);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float4 a = *reinterpret_cast<const float4 *>(&A[r0 + i][k]);
+                    const float av[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                    for (int j = 0; j < 4; j++) { acc[i].x += av[j] * b[j].x; acc[i].y += av[j] * b[j].y; acc[i].z += av[j] * b[j].z; acc[i].w += av[j] * b[j].w; }
+                }
             }
+#pragma unroll
+            for (int i = 0; i < 8; i++) parts[(warp * 8 + i) * 32 + lane] = acc[i];
+            __syncthreads();
+            const uint32_t r = r0 + (warp & 7u), c = lane * 4, side = warp >> 3, some = ranks / 2;
+            float4 s = make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (uint32_t w = 0; w < NS_WARPS; w++) { const float4 v = parts[(w * 8 + (warp & 7u)) * 32 + lane]; s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w; }
             const float4 q = *reinterpret_cast<const float4 *>(&A[r][c]);
             s.x = NS_B * q.x + NS_C * s.x + (r == c ? NS_A : 0.0f); s.y = NS_B * q.y + NS_C * s.y + (r == c + 1 ? NS_A : 0.0f);
             s.z = NS_B * q.z + NS_C * s.z + (r == c + 2 ? NS_A : 0.0f); s.w = NS_B * q.w + NS_C * s.w + (r == c + 3 ? NS_A : 0.0f);
 #pragma unroll 8
-            for (uint32_t t = 0; t < ranks; t++) remote4(&B[r][c], t, s);
+            for (uint32_t t = side * some; t < (side + 1) * some; t++) remote4(&B[r][c], t, s);
+            __syncthreads();
         }
         hg::cluster_sync();
-        {   // X_r = B X_r: 4 rows x 4 columns a thread; B is symmetric, so its rows are read as columns
-            const uint32_t r0 = (tid & 31u) * 4, q0 = (tid >> 5) * 4;
-            float acc[4][4] = {};
+        {   // X_r = B X_r: 4 rows x 2 columns a thread; B is symmetric to rounding, so its rows are read as columns
+            const uint32_t r0 = lane * 4, q0 = warp * 2;
+            float acc[2][4] = {};
             if (q0 < mine) {
-#pragma unroll 4
-                for (uint32_t k = 0; k < m; k++) {
-                    const float4 b = *reinterpret_cast<const float4 *>(&B[k][r0]);
-                    const float x[4] = {X[q0][k], X[q0 + 1][k], X[q0 + 2][k], X[q0 + 3][k]};
+#pragma unroll 2
+                for (uint32_t k = 0; k < m; k += 4) {      // (rows and columns beyond m are zeros)
+                    const float4 x0 = *reinterpret_cast<const float4 *>(&X[q0][k]), x1 = *reinterpret_cast<const float4 *>(&X[q0 + 1][k]);
+                    const float u[4] = {x0.x, x0.y, x0.z, x0.w}, v[4] = {x1.x, x1.y, x1.z, x1.w};
 #pragma unroll
-                    for (int j = 0; j < 4; j++) { acc[j][0] += b.x * x[j]; acc[j][1] += b.y * x[j]; acc[j][2] += b.z * x[j]; acc[j][3] += b.w * x[j]; }
+                    for (int j = 0; j < 4; j++) {
+                        const float4 b = *reinterpret_cast<const float4 *>(&B[k + j][r0]);
+                        acc[0][0] += b.x * u[j]; acc[0][1] += b.y * u[j]; acc[0][2] += b.z * u[j]; acc[0][3] += b.w * u[j];
+                        acc[1][0] += b.x * v[j]; acc[1][1] += b.y * v[j]; acc[1][2] += b.z * v[j]; acc[1][3] += b.w * v[j];
+                    }
                 }
             }
             __syncthreads();
             if (q0 < mine)
 #pragma unroll
-                for (int j = 0; j < 4; j++) *reinterpret_cast<float4 *>(&X[q0 + j][r0]) = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
+                for (int j = 0; j < 2; j++) *reinterpret_cast<float4 *>(&X[q0 + j][r0]) = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
         }
     }
     __syncthreads();
@@ -298,7 +323,7 @@ static uint32_t ns_small_ranks(uint32_t m, uint32_t n) {
         cudaLaunchAttribute a[1];
         a[0].id = cudaLaunchAttributeClusterDimension;
         a[0].val.clusterDim.x = 1; a[0].val.clusterDim.y = 16; a[0].val.clusterDim.z = 1;
-        c.gridDim = dim3(1, 16); c.blockDim = dim3(256); c.dynamicSmemBytes = NS_SMEM; c.attrs = a; c.numAttrs = 1;
+        c.gridDim = dim3(1, 16); c.blockDim = dim3(NS_THREADS); c.dynamicSmemBytes = NS_SMEM; c.attrs = a; c.numAttrs = 1;
         int clusters = 0;
         if (cudaOccupancyMaxActiveClusters(&clusters, k_ns_small, &c) == cudaSuccess && clusters > 0) most = 16;
         else cudaGetLastError();
@@ -314,7 +339,7 @@ static bool newton_schulz(float *out, float *param, float *mom, const float *gra
     if (const uint32_t ranks = ns_small_ranks(m, k)) {
         layer_estimate(2.0 * steps * m * m * (2.0 * k + m), 4.0 * rows * cols * (param ? 5 : 2));
         profile_begin();
-        chain_cluster(ranks, k_ns_small, dim3(1, ranks), 256, NS_SMEM, NsSmall{out, param, mom, grad, rows, cols, steps, nesterov, mu, keep, step});
+        chain_cluster(ranks, k_ns_small, dim3(1, ranks), NS_THREADS, NS_SMEM, NsSmall{out, param, mom, grad, rows, cols, steps, nesterov, mu, keep, step});
         after_launch("newton_schulz_small");
         return true;
     }
