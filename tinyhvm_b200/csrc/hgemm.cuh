@@ -9,7 +9,7 @@
 // product is below 2^-24): three f16 MMAs, where three tf32 MMAs would run at half their rate and keep 2^-21.
 //
 // The tensor core truncates when it adds to an accumulator, so a long sum drifts towards zero by about 2^-24 per add.
-// Here an accumulator lives for 128 k only (1024 without low planes): eight epilogue warps then take it from
+// Here an accumulator lives for 128 k only (1024 or 2048 without low planes): eight epilogue warps then take it from
 // tensor memory and add it, rounded, to f32 sums in registers, while the MMAs of the next chunk fill the other of
 // two accumulators.  Within a block of k the small products go first.
 //
@@ -20,6 +20,11 @@
 //
 // Operands may lie either way round, as the matrix descriptors allow for f16: k along memory rows (boxes of 64 k x rows),
 // or m / n along memory rows (boxes of 64 rows x 64 k), so nothing is ever transposed.
+//
+// What bounds it, measured: the tensor cores, and the power they draw.  8192 x 4096 x 4096 in f16 207 us, 1326 TFLOP/s, 0.80 of the measured
+// burst rate (in a loop the clock falls to 1.35 GHz: 250 us); 4096^3 in f32 358 us with the planes' making, 385 TFLOP/s, of which
+// three f16 MMAs each make 1154.  A pair takes 1900 cycles for 64 k of three products, whose MMAs take 1536: the rest is the epilogue where the
+// next tile's first two chunks do not hide it, and tile loads and MMAs sharing shared memory's bandwidth (without loads 1640).
 //
 // Every wait is bounded.  A wait that runs out raises status bit 8 and ends the kernel after its copies in flight.
 #pragma once
@@ -144,6 +149,10 @@ __device__ __forceinline__ void acc_load(uint32_t addr, uint32_t (&r)[32]) {
 template <typename T> __device__ __forceinline__ void touch_row(const T *row, uint32_t from, uint32_t n, uint32_t end) {
     for (uint32_t i = from; i < from + n && i < end; i += 128u / sizeof(T)) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + i));
 }
+
+// The chunks of a tile.  Without low planes the first two are twice as long, so that the MMAs have work while the epilogue warps finish the
+// tile before.  (With them that gains 8% at K = 1024, but sums of one sign would be off by 1.6e-6 instead of 0.6e-6.)
+__device__ __forceinline__ uint32_t chunk_end(uint32_t kb, uint32_t chunk) { return kb + (chunk > 2u && kb < 4 * chunk ? 2 * chunk : chunk); }
 
 struct Tile { uint32_t m0, n0, z, blocks, block0; };
 // Tiles in order: split, then bands of 8 row tiles, columns, rows of the band: the tiles in flight share few operand panels.
@@ -294,7 +303,7 @@ k_hgemm(const __grid_constant__ Shape S, const __grid_constant__ Maps maps, cons
             float acc[COLS];
 #pragma unroll
             for (uint32_t i = 0; i < COLS; i++) acc[i] = 0.0f;
-            for (uint32_t kb = 0; kb < T.blocks && ok; kb += S.chunk, c++) {
+            for (uint32_t kb = 0; kb < T.blocks && ok; kb = chunk_end(kb, S.chunk), c++) {
                 const uint32_t buf = c & 1u;
                 ok = bar_wait(smem32(&sh.acc_full[buf]), (c >> 1) & 1u, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
@@ -384,10 +393,10 @@ k_hgemm(const __grid_constant__ Shape S, const __grid_constant__ Maps maps, cons
             uint64_t at = 0;                               // of the stage, in the descriptors' units
             for (uint32_t t = pair; t < S.tiles && ok; t += pairs) {
                 const Tile T = tile_of<NT>(S, t);
-                for (uint32_t kb = 0; kb < T.blocks && ok; kb += chunk, c++) {
+                for (uint32_t kb = 0; kb < T.blocks && ok; kb = chunk_end(kb, chunk), c++) {
                     const uint32_t buf = c & 1u, d = tmem + buf * NT;
                     if (c >= 2) ok = bar_spin(smem32(&sh.acc_empty[buf]), ((c >> 1) - 1) & 1u, abort_flag);
-                    const uint32_t end = T.blocks - kb < chunk ? T.blocks - kb : chunk;
+                    const uint32_t next = chunk_end(kb, chunk), end = (next < T.blocks ? next : T.blocks) - kb;
                     uint32_t more = 0;
                     for (uint32_t i = 0; i < end && ok; i++) {
                         ok = bar_spin(smem32(&sh.full[s]), use & 1u, abort_flag);

@@ -5,7 +5,8 @@
 //   dx = rstd (g - sum g / cols - xh sum(g xh) / cols),  dgamma = sum_rows dy xh,  dbeta = sum_rows dy
 //
 // All sums are f32 over f32 values whatever the storage type; only the stored results are rounded.  Both passes are
-// bound by memory: forward reads x and writes y, backward reads x and dy and writes dx, each once.
+// bound by memory: forward reads x and writes y, backward reads x and dy and writes dx, each once.  16384 x 2048 f32: forward 45 us,
+// 5.98 TB/s, 0.91 of the measured copy rate; backward 70 us, 5.73 TB/s, 0.87 (7 us of it add up 592 blocks' partial sums).
 //
 // A row belongs to a group of G threads, which keeps it in registers from the load to the store, so the deviation from
 // the mean is summed in a second pass that costs no memory traffic.  The backward pass keeps, beside the row, the running

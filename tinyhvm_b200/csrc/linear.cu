@@ -2,6 +2,11 @@
 //
 //   forward   z = x w + bias,  y = act(z) + residual                    x [M,K], w [K,N] (in, out: as the framework stores weights)
 //   backward  dz = dy act'(z);  dx = dz w^T;  dw = x^T dz;  dbias = sum over rows of dz
+//
+// Three ways, by size: a few rows on the CUDA cores with the weights streamed once (k_linear_few); small products in one launch on the CUDA
+// cores (layer_small.cuh); the rest on the matrix engine (hgemm.cuh), f16 operands as they lie in memory, f32 ones as two f16 planes that
+// kernels of this file make first.  Forward 4096 x 1024 -> 4096, f32, gelu, z kept: 136 us, 17 of them the planes; its backward pass
+// 255 us: dz and its planes 40, x's 31, w's 8, bias 7, the two products 166.
 #include "hgemm.cuh"
 #include "layer_common.cuh"
 #include "layer_host.h"
