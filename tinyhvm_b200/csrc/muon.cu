@@ -4,7 +4,7 @@
 // with the quintic's coefficients a, b, c = 3.4445, -4.7750, 2.0315: X keeps G's singular vectors and its singular values
 // move to the neighbourhood of 1.
 // On the matrix engine a step is three products, with the matrices between them kept as the engine's f16 planes: A and B are symmetric and
-// only made from the diagonal on, and B takes a I in, so that X = B X needs no other read.  Five steps: 4096 x 4096 3.7 ms (1374 GFLOP with
+// only made from the diagonal on.  Five steps: 4096 x 4096 3.7 ms (1374 GFLOP with
 // the symmetry used: 375 TFLOP/s, 1125 of f16 products, the clock at its power limit); 1024 x 4096 370 us.
 //   mom = mu mom + g;  u = nesterov ? g + mu mom : mom;  p = p (1 - lr decay) - lr sqrt(max(1, rows / cols)) X(u)
 #include <math.h>
@@ -17,8 +17,8 @@ namespace thc {
 
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 
-// Planes hold 2^13 times the value: X and its square stay below 1.5 in magnitude, the polynomial below 3.45, so the largest is
-// 28262 and the low part's step is 2^-37.
+// Planes hold 2^13 times the value: X and its square stay below 1.5 in magnitude, b A + c A A below 2.9, so the largest is below 24000 and the
+// low part's step is 2^-37.
 constexpr float PLANE = 8192.0f;
 
 // mom = mu mom + grad (when there is a momentum) and the sum of squares of the update: one partial per block, in double, which
@@ -108,7 +108,7 @@ struct SquareEpi {                                     // A = X X^T
     template <int V, int R> __device__ void put(hg::Rows r, uint32_t n, float (&v)[R][V], const float (&)[R][V], uint32_t) const { put_planes<V, R>(hi, lo, pitch, r, n, v); }
     template <int V, int R> __device__ void mirror(hg::Rows r, uint32_t m, const float (&v)[R][V]) const { put_planes<V, R>(hi, lo, pitch, r, m, v); }
 };
-struct PolyEpi {                                       // a I + b A + c A A
+struct PolyEpi {                                       // b A + c A A
     static constexpr bool mirrors = true;
     __half *hi, *lo; const __half *a_hi, *a_lo; uint64_t pitch; uint32_t side;
     __device__ bool wide() const { return side % 4 == 0; }
@@ -126,33 +126,43 @@ struct PolyEpi {                                       // a I + b A + c A A
 #pragma unroll
         for (uint32_t i = 0; i < R; i++)
 #pragma unroll
-            for (int j = 0; j < V; j++) v[i][j] = NS_B * x[i][j] + NS_C * v[i][j] + (r.first + i * r.step == n + j ? NS_A * PLANE : 0.0f);
+            for (int j = 0; j < V; j++) v[i][j] = NS_B * x[i][j] + NS_C * v[i][j];
         put_planes<V, R>(hi, lo, pitch, r, n, v);
     }
     template <int V, int R> __device__ void mirror(hg::Rows r, uint32_t m, const float (&v)[R][V]) const { put_planes<V, R>(hi, lo, pitch, r, m, v); }
 };
 enum { NEXT, RESULT, STEP };
-template <int TO> struct ApplyEpi {                    // X = (a I + b A + c A A) X: planes for the next step, the result, or the parameters' step
+// X = a X + (b A + c A A) X: planes for the next step, the result, or the parameters' step.  a X is added here, in f32: it is most of the sum
+// while the small singular values still grow, and the tensor core's truncation would be a share of it.
+template <int TO> struct ApplyEpi {
     static constexpr bool mirrors = false;
-    __half *hi, *lo; uint64_t pitch;
+    const __half *x_hi, *x_lo; __half *hi, *lo; uint64_t pitch;
     float *out; uint32_t cols; float keep, step;
     __device__ bool wide() const { return cols % 4 == 0; }
     __device__ void touch(uint32_t m, uint32_t n, uint32_t count) const { if constexpr (TO == STEP) hg::touch_row(out + (uint64_t)m * cols, n, count, cols); }
     __device__ float row_factor(uint32_t) const { return TO == NEXT ? 1.0f / PLANE : 1.0f / (PLANE * PLANE); }
     template <int V> __device__ void column(uint32_t) const {}
-    template <int V> __device__ void fetch(uint32_t m, uint32_t n, float (&x)[V]) const { if constexpr (TO == STEP) load_vec<V>(out + (uint64_t)m * cols + n, x); }
+    template <int V> __device__ void fetch(uint32_t m, uint32_t n, float (&x)[V]) const {
+        float l[V], p[V];
+        load_vec<V>(x_hi + m * pitch + n, x);
+        load_vec<V>(x_lo + m * pitch + n, l);
+        if constexpr (TO == STEP) load_vec<V>(out + (uint64_t)m * cols + n, p);
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            x[j] = (x[j] + l[j]) * (TO == NEXT ? NS_A : NS_A / PLANE);
+            if constexpr (TO == STEP) x[j] = p[j] * keep - step * x[j];
+        }
+    }
     template <int V, int R> __device__ void put(hg::Rows r, uint32_t n, float (&v)[R][V], const float (&x)[R][V], uint32_t) const {
+#pragma unroll
+        for (int i = 0; i < R; i++)
+#pragma unroll
+            for (int j = 0; j < V; j++) v[i][j] = TO == STEP ? x[i][j] - step * v[i][j] : x[i][j] + v[i][j];
         if constexpr (TO == NEXT) { put_planes<V, R>(hi, lo, pitch, r, n, v); return; }
         float *p = out + (uint64_t)r.first * cols + n;
         const uint64_t down = (uint64_t)r.step * cols;
 #pragma unroll
-        for (uint32_t i = 0; i < R; i++, p += down) {
-            if constexpr (TO == STEP) {
-#pragma unroll
-                for (int j = 0; j < V; j++) v[i][j] = x[i][j] * keep - step * v[i][j];
-            }
-            if (r.first + i * r.step < r.end) store_vec<V>(p, v[i]);
-        }
+        for (uint32_t i = 0; i < R; i++, p += down) if (r.first + i * r.step < r.end) store_vec<V>(p, v[i]);
     }
 };
 
@@ -377,9 +387,9 @@ static bool newton_schulz(float *out, float *param, float *mom, const float *gra
         hg::product(A, A, m, m, m, poly, partial, PolyEpi{b[0], b[1], a[0], a[1], pm, m}, true, "newton_schulz_poly");
         const hg::Operand Xr{cur[0], px, rows * px, wide};                     // X across: the other way round than in its square
         const auto run = [&](auto epi) { hg::product(wide ? B : Xr, wide ? Xr : B, rows, cols, m, apply, partial, epi, false, "newton_schulz_apply"); };
-        if (i + 1 < steps) run(ApplyEpi<NEXT>{next[0], next[1], px, nullptr, cols, 0.0f, 0.0f});
-        else if (param) run(ApplyEpi<STEP>{nullptr, nullptr, 0, param, cols, keep, step});
-        else run(ApplyEpi<RESULT>{nullptr, nullptr, 0, out, cols, 0.0f, 0.0f});
+        if (i + 1 < steps) run(ApplyEpi<NEXT>{cur[0], cur[1], next[0], next[1], px, nullptr, cols, 0.0f, 0.0f});
+        else if (param) run(ApplyEpi<STEP>{cur[0], cur[1], nullptr, nullptr, px, param, cols, keep, step});
+        else run(ApplyEpi<RESULT>{cur[0], cur[1], nullptr, nullptr, px, out, cols, 0.0f, 0.0f});
     }
     return true;
 }
