@@ -2,9 +2,10 @@
 
 Tolerances.  A stored value is off by half a step, HALF[dtype] relative (f32 2^-24, f16 2^-11), and below the smallest normal
 f16 by 2^-25 absolute.  A sum of K products in f32 with S = sum |a b| is off by at most (C + K / 32) 2^-24 S here: the operands'
-representation costs 3 x 2^-24, runs of at most 128 terms go through the tensor core, whose truncating adds cost 2^-23 each
-and are 24 at most per run, and the runs are added with rounding; sums of K terms on the CUDA cores split K over 32 lanes
-or more, or have K at most 64 terms in a row: C = 64 covers both.  Random signs keep the whole output far below that, so its 2-norm is
+representation costs 3 x 2^-24, runs of at most 128 terms go through the tensor core, whose truncating adds cost up to 2^-23 of what has
+been summed each and are 24 at most per run (half of S on average: 24 x 2^-24), and the runs are added with rounding; sums of
+K terms on the CUDA cores have at most 64 terms in a row: C = 64 covers both.  (f16 operands have runs of 2048 terms and 128 adds,
+which is nothing beside their results' own rounding: HALF is 8192 times as much.)  Random signs keep the whole output far below that, so its 2-norm is
 held to 2e-6 as well: a product that lost one of its operands' low parts would be 2e-5 off or more.
 """
 import ctypes as C
@@ -276,6 +277,23 @@ def test_linear_backward_parts_are_the_whole(host):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", [F32, F16])
+@pytest.mark.parametrize("M,K,N", [(3, 5, 7), (130, 200, 96), (520, 640, 704), (300, 700, 9001)])
+def test_linear_backward_without_what_it_does_not_need(host, M, K, N, dt):
+    """dx needs no x, dw no w, dbias neither, and none of them z without an activation."""
+    rng = np.random.default_rng(M)
+    dy, x, w = (rng.standard_normal(s).astype(NP[dt]) for s in ((M, N), (M, K), (K, N)))
+    bdy, bx, bw = host.up(dy), host.up(x), host.up(w)
+    bdx, bdw, bdb = host.out(M * K, dt), host.out(K * N, dt), host.out(N, dt)
+    call = host.lib.thvm_cuda_linear_backward
+    assert call(bdx, 0, 0, bdy, 0, 0, bw, M, K, N, NONE, dt) == 0 and call(0, bdw, 0, bdy, 0, bx, 0, M, K, N, NONE, dt) == 0 and call(0, 0, bdb, bdy, 0, 0, 0, M, K, N, NONE, dt) == 0
+    dy, x, w = (a.astype(np.float64) for a in (dy, x, w))
+    for bid, want, S, n in ((bdx, dy @ w.T, np.abs(dy) @ np.abs(w).T, N), (bdw, x.T @ dy, np.abs(x).T @ np.abs(dy), M), (bdb, dy.sum(0), np.abs(dy).sum(0), M)):
+        near(host.get(bid, want.shape, dt).astype(np.float64), want, product_slack(n, S) + HALF[dt] * np.abs(want) * 1.01 + TINY[dt])
+    host.done()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F32, F16])
 @pytest.mark.parametrize("M,K,N", [(1, 64, 100), (70, 300, 72), (300, 520, 520)])
 def test_linear_residual_in_place(host, M, K, N, dt):
     """y in the residual's own buffer, twice: the second call adds to what the first left."""
@@ -428,7 +446,7 @@ def test_layernorm_of_large_means_and_constant_rows(host):
 
 
 # ---- Newton-Schulz ----
-MATRICES = [(1, 1), (1, 50), (50, 1), (8, 8), (10, 84), (84, 10), (120, 84), (400, 120), (96, 97), (128, 256), (130, 520), (520, 264), (300, 300), (128, 512), (129, 400), (100, 513), (200, 2100), (1100, 150), (600, 601)]
+MATRICES = [(1, 1), (1, 50), (50, 1), (8, 8), (10, 84), (84, 10), (120, 84), (400, 120), (96, 97), (128, 256), (130, 520), (520, 264), (300, 300), (128, 512), (129, 400), (100, 513), (57, 1100), (128, 1536), (1537, 90), (700, 128), (200, 2100), (1100, 150), (600, 601)]
 
 
 def spread(rng, rows, cols):

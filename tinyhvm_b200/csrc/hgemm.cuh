@@ -62,7 +62,7 @@ constexpr size_t SMEM = 1024 + RING_BYTES + STAGING + sizeof(Shared);
 struct Shape {
     uint32_t M, N, K;
     uint32_t row_tiles, col_tiles, tiles;                  // tiles: of all splits, below the diagonal left out when `upper`
-    uint32_t blocks, split_blocks, chunk;                  // blocks of k: in all, per split, per chunk
+    uint32_t blocks, split_blocks, chunk, lead;            // blocks of k: in all, per split, per chunk; how much longer a tile's first two are
     uint32_t split_tiles;                                  // tiles of a split
     uint32_t halves, stages, stage_bytes, half_bytes, a_bytes;   // a block of k is one or two times 64 k: a half holds A's and B's planes of 64 k
     uint32_t a_mode, b_mode, a_lo, b_lo, upper;
@@ -150,9 +150,10 @@ template <typename T> __device__ __forceinline__ void touch_row(const T *row, ui
     for (uint32_t i = from; i < from + n && i < end; i += 128u / sizeof(T)) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + i));
 }
 
-// The chunks of a tile.  Without low planes the first two are twice as long, so that the MMAs have work while the epilogue warps finish the
-// tile before.  (With them that gains 8% at K = 1024, but sums of one sign would be off by 1.6e-6 instead of 0.6e-6.)
-__device__ __forceinline__ uint32_t chunk_end(uint32_t kb, uint32_t chunk) { return kb + (chunk > 2u && kb < 4 * chunk ? 2 * chunk : chunk); }
+// The chunks of a tile: the first two are `lead` times as long, so that the MMAs have work while the epilogue warps finish the tile before.
+// Twice, without low planes or where the epilogue adds more than the product is (Epi::long_start); else once: twice gains 8% at
+// K = 1024, but sums of one sign would be off by 1.6e-6 instead of 0.6e-6.
+__device__ __forceinline__ uint32_t chunk_end(uint32_t kb, uint32_t chunk, uint32_t lead) { return kb + (kb < 2 * lead * chunk ? lead * chunk : chunk); }
 
 struct Tile { uint32_t m0, n0, z, blocks, block0; };
 // Tiles in order: split, then bands of 8 row tiles, columns, rows of the band: the tiles in flight share few operand panels.
@@ -303,7 +304,7 @@ k_hgemm(const __grid_constant__ Shape S, const __grid_constant__ Maps maps, cons
             float acc[COLS];
 #pragma unroll
             for (uint32_t i = 0; i < COLS; i++) acc[i] = 0.0f;
-            for (uint32_t kb = 0; kb < T.blocks && ok; kb = chunk_end(kb, S.chunk), c++) {
+            for (uint32_t kb = 0; kb < T.blocks && ok; kb = chunk_end(kb, S.chunk, S.lead), c++) {
                 const uint32_t buf = c & 1u;
                 ok = bar_wait(smem32(&sh.acc_full[buf]), (c >> 1) & 1u, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
@@ -386,17 +387,17 @@ k_hgemm(const __grid_constant__ Shape S, const __grid_constant__ Maps maps, cons
             const uint32_t a_mn = S.a_mode != K_ROWS, b_mn = S.b_mode != K_ROWS;
             const uint32_t idesc = (1u << 4) | (a_mn << 15) | (b_mn << 16) | ((NT >> 3) << 17) | ((256u >> 4) << 24);   // f32 sums of f16 products
             const uint64_t step_a = a_mn ? 2048u >> 4 : 32u >> 4, step_b = b_mn ? 2048u >> 4 : 32u >> 4;                 // 16 k further
-            const uint32_t lo = S.a_lo | S.b_lo << 1, halves = S.halves, chunk = S.chunk, stages = S.stages;
+            const uint32_t lo = S.a_lo | S.b_lo << 1, halves = S.halves, chunk = S.chunk, lead = S.lead, stages = S.stages;
             const uint64_t a_first = operand_desc(ring, a_mn), b_first = operand_desc(ring + S.a_bytes, b_mn), half = S.half_bytes >> 4;
             bool ok = true;
             uint32_t s = 0, use = 0, c = 0;
             uint64_t at = 0;                               // of the stage, in the descriptors' units
             for (uint32_t t = pair; t < S.tiles && ok; t += pairs) {
                 const Tile T = tile_of<NT>(S, t);
-                for (uint32_t kb = 0; kb < T.blocks && ok; kb = chunk_end(kb, chunk), c++) {
+                for (uint32_t kb = 0; kb < T.blocks && ok; kb = chunk_end(kb, chunk, lead), c++) {
                     const uint32_t buf = c & 1u, d = tmem + buf * NT;
                     if (c >= 2) ok = bar_spin(smem32(&sh.acc_empty[buf]), ((c >> 1) - 1) & 1u, abort_flag);
-                    const uint32_t next = chunk_end(kb, chunk), end = (next < T.blocks ? next : T.blocks) - kb;
+                    const uint32_t next = chunk_end(kb, chunk, lead), end = (next < T.blocks ? next : T.blocks) - kb;
                     uint32_t more = 0;
                     for (uint32_t i = 0; i < end && ok; i++) {
                         ok = bar_spin(smem32(&sh.full[s]), use & 1u, abort_flag);
@@ -438,7 +439,7 @@ k_hgemm(const __grid_constant__ Shape S, const __grid_constant__ Maps maps, cons
 
 // Sums of a split product: partial[z][m][n] in split order, then the epilogue.
 struct PartialEpi {
-    static constexpr bool mirrors = false;
+    static constexpr bool mirrors = false, long_start = false;
     float *partial; uint64_t mn; uint32_t N;
     __device__ bool wide() const { return N % 4 == 0; }
     __device__ float row_factor(uint32_t) const { return 1.0f; }
@@ -612,6 +613,7 @@ static void product(const Operand &A, const Operand &B, uint32_t M, uint32_t N, 
     const uint32_t splits = (S.blocks + S.split_blocks - 1) / S.split_blocks;          // p.splits or fewer
     S.a_lo = A.plane != 0; S.b_lo = B.plane != 0;
     S.chunk = S.a_lo || S.b_lo ? 2 : 8;
+    S.lead = !(S.a_lo || S.b_lo) || Epi::long_start ? 2 : 1;
     S.a_bytes = A_PLANE * (1 + S.a_lo);
     S.half_bytes = S.a_bytes + p.nt / 2 * 128 * (1 + S.b_lo);
     S.stage_bytes = S.half_bytes * S.halves;

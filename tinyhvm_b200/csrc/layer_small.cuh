@@ -52,7 +52,7 @@ __device__ __forceinline__ void small_tile(const Small<T> &S, SmallShared &sh, u
         for (uint32_t i = 0; i < 16; i++) {                // lanes run along memory
             if constexpr (MODE == SMALL_Y) ra[i] = small_at(S.x, r0 + warp + 4 * i, d + lane, S.M, S.K);
             if constexpr (MODE == SMALL_DX) ra[i] = small_dz(S, r0 + warp + 4 * i, d + lane);
-            if constexpr (MODE == SMALL_DW) ra[i] = small_at(S.x, d + warp + 4 * (i & 7), r0 + (i >> 3) * 32 + lane, S.M, S.K);
+            if constexpr (MODE == SMALL_DW) ra[i] = S.dw ? small_at(S.x, d + warp + 4 * (i & 7), r0 + (i >> 3) * 32 + lane, S.M, S.K) : 0.0f;    // (for dbias alone there need be no x)
         }
 #pragma unroll
         for (uint32_t i = 0; i < 8; i++) {

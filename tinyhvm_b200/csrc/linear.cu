@@ -278,7 +278,7 @@ template <typename T, int V, int R> __device__ __forceinline__ void store_rows(T
     for (uint32_t i = 0; i < R; i++, p += step) if (r.first + i * r.step < r.end) store_vec<V>(p, v[i]);
 }
 template <typename T, uint32_t ACT> struct LayerEpi {  // act(sum 2^-exps[m] + bias) + residual
-    static constexpr bool mirrors = false;
+    static constexpr bool mirrors = false, long_start = false;
     T *out, *z; const T *bias, *residual; const int *exps; uint32_t N;
     float bias_n[4];                                   // of the lane's columns
     __device__ bool wide() const { return N % 4 == 0; }
@@ -303,7 +303,7 @@ template <typename T, uint32_t ACT> struct LayerEpi {  // act(sum 2^-exps[m] + b
     }
 };
 template <typename T, bool COLS> struct GradEpi {      // sum 2^(-exps[m] - col_exps[n])
-    static constexpr bool mirrors = false;
+    static constexpr bool mirrors = false, long_start = false;
     T *out; const int *exps, *col_exps; uint32_t N;
     int exp_n[4];
     __device__ bool wide() const { return N % 4 == 0; }
@@ -480,17 +480,18 @@ template <typename T> static bool few_rows(void *y, void *z, const void *x, cons
 }
 
 // Up to how many products (M K N) the one-launch kernels of layer_small.cuh are taken.  Forward, f32: 512 x 400 x 120 in 9 us, the engine with its
-// operands' planes 16; 512 x 512 x 512 in 20 and 18; in f16 the engine needs no planes and is as fast at 64 x 64 x 64 (6 us).  Backward:
+// operands' planes 16; 512 x 512 x 512 in 20 and 18; in f16 the engine needs no planes and is as fast at 64 x 64 x 64 (6 us), except for rows
+// that it has to copy to an aligned pitch first (265 x 177 x 221 18 us).  Backward:
 // f32 256^3 12 and 31 us, 512 x 400 x 120 22 and 35, 1024 x 400 x 120 44 and 37; f16 17 and 27, 29 and 30; with 2000 rows, over which dw sums,
 // 32 and 34, 49 and 32.
-constexpr double SMALL_FORWARD = 1e8, SMALL_BACKWARD_F32 = 4e7, SMALL_BACKWARD_F16 = 2e7;
+constexpr double SMALL_FORWARD = 1e8, SMALL_FORWARD_COPIED = 2e7, SMALL_BACKWARD_F32 = 4e7, SMALL_BACKWARD_F16 = 2e7;
 constexpr uint32_t SMALL_BACKWARD_ROWS = 1024;
 
 template <typename T>
 static bool linear_forward(void *y, void *z, const void *x, const void *w, const void *bias, const void *residual, uint32_t M, uint32_t K, uint32_t N, uint32_t act) {
     constexpr bool F = sizeof(T) == 4;
     if (few_rows<T>(y, z, x, w, bias, residual, M, K, N, act)) return true;
-    if constexpr (F) if ((double)M * K * N <= SMALL_FORWARD) {
+    if ((double)M * K * N <= (F ? SMALL_FORWARD : K % 8 || N % 8 ? SMALL_FORWARD_COPIED : 0)) {
         Small<T> S{};
         S.x = (const T *)x; S.w = (const T *)w; S.bias = (const T *)bias; S.residual = (const T *)residual; S.y = (T *)y; S.z_out = (T *)z;
         S.M = M; S.K = K; S.N = N; S.act = act;

@@ -98,7 +98,7 @@ template <int V, int R> __device__ __forceinline__ void put_planes(__half *hi, _
     for (uint32_t i = 0; i < R; i++) if (r.first + i * r.step < r.end) store_planes<V>(hi + at + i * step, lo + at + i * step, v[i]);
 }
 struct SquareEpi {                                     // A = X X^T
-    static constexpr bool mirrors = true;
+    static constexpr bool mirrors = true, long_start = false;
     __half *hi, *lo; uint64_t pitch; uint32_t side;
     __device__ bool wide() const { return side % 4 == 0; }
     __device__ float row_factor(uint32_t) const { return 1.0f / PLANE; }
@@ -109,7 +109,7 @@ struct SquareEpi {                                     // A = X X^T
     template <int V, int R> __device__ void mirror(hg::Rows r, uint32_t m, const float (&v)[R][V]) const { put_planes<V, R>(hi, lo, pitch, r, m, v); }
 };
 struct PolyEpi {                                       // b A + c A A
-    static constexpr bool mirrors = true;
+    static constexpr bool mirrors = true, long_start = false;
     __half *hi, *lo; const __half *a_hi, *a_lo; uint64_t pitch; uint32_t side;
     __device__ bool wide() const { return side % 4 == 0; }
     __device__ float row_factor(uint32_t) const { return 1.0f / PLANE; }
@@ -135,7 +135,7 @@ enum { NEXT, RESULT, STEP };
 // X = a X + (b A + c A A) X: planes for the next step, the result, or the parameters' step.  a X is added here, in f32: it is most of the sum
 // while the small singular values still grow, and the tensor core's truncation would be a share of it.
 template <int TO> struct ApplyEpi {
-    static constexpr bool mirrors = false;
+    static constexpr bool mirrors = false, long_start = true;
     const __half *x_hi, *x_lo; __half *hi, *lo; uint64_t pitch;
     float *out; uint32_t cols; float keep, step;
     __device__ bool wide() const { return cols % 4 == 0; }
@@ -167,14 +167,15 @@ template <int TO> struct ApplyEpi {
 };
 
 // ---- small matrices: one launch, everything in one cluster's shared memory ----
-// The smaller side is at most 128, the larger 32 times the cluster.  Block r of the cluster keeps every row of its own share of the larger
+// The smaller side is at most 128, the larger 64 times the cluster (128 x 1024 157 us, 128 x 1536 205; on
+// the engine 128 x 1600 177).  Block r of the cluster keeps every row of its own share of the larger
 // side's columns, X_r (stored column by column), and A and B whole.  A step: P_r = X_r X_r^T by each block; A = sum of P_r, an equal share
 // of rows by each block, written to all; B = a I + b A + c A A the same way; X_r = B X_r.  Three barriers of the cluster a step.  All in
 // f32 on the CUDA cores: 0.03 GFLOP a step at 400 x 120 is nothing; what bounds it is the latency of the shared-memory reads with four warps a
 // scheduler and of the exchange: 400 x 120, five steps, 100 us, of a step's 38000 cycles 8000 in the barriers, 8000 in adding and
 // spreading A, 6000 in each of P and B, 9000 in B X.  As 15 launches of the matrix engine it takes 164 us.
-constexpr uint32_t NS_SIDE = 128, NS_SHARE = 32, NS_PITCH = 132, NS_THREADS = 512, NS_WARPS = NS_THREADS / 32;
-constexpr size_t NS_SMEM = (size_t)(NS_SHARE + 2 * NS_SIDE) * NS_PITCH * 4 + (size_t)NS_WARPS * 8 * NS_SIDE * 4;     // X, A, B; the warps' parts of B's rows
+constexpr uint32_t NS_SIDE = 128, NS_SHARE = 64, NS_PITCH = 132, NS_THREADS = 512, NS_WARPS = NS_THREADS / 32;
+constexpr size_t NS_SMEM = (size_t)(NS_SHARE + 2 * NS_SIDE) * NS_PITCH * 4 + 32 * NS_SIDE * 4;     // X, A, B; parts of eight rows
 struct NsSmall { float *out, *param, *mom; const float *grad; uint32_t rows, cols, steps; int nesterov; float mu, keep, step; };
 
 __device__ __forceinline__ float4 remote4(const float *p, uint32_t rank) {
@@ -191,16 +192,17 @@ k_ns_small(const __grid_constant__ NsSmall S) {
     extern __shared__ __align__(16) float ns[];
     float (*X)[NS_PITCH] = reinterpret_cast<float (*)[NS_PITCH]>(ns);                              // [NS_SHARE]: column, row
     float (*A)[NS_PITCH] = X + NS_SHARE, (*B)[NS_PITCH] = A + NS_SIDE;                             // [NS_SIDE]; B first holds P
-    float4 *parts = reinterpret_cast<float4 *>(B + NS_SIDE);                                       // [NS_WARPS][8][32]
+    float4 *parts = reinterpret_cast<float4 *>(B + NS_SIDE);                                       // [4][8][32]
     __shared__ double red[NS_WARPS], norm;
     const uint32_t ranks = gridDim.y, rank = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const bool wide = S.rows <= S.cols;
     const uint32_t m = wide ? S.rows : S.cols, n = wide ? S.cols : S.rows, share = (n + ranks - 1) / ranks;
     const uint32_t c0 = rank * share, mine = c0 >= n ? 0 : n - c0 < share ? n - c0 : share;        // columns c0 .. c0 + mine
+    const uint32_t padded = (share + 31u) & ~31u;          // columns kept: whole groups of 32
     // the update, its place in memory and its sum of squares; rows and columns beyond the matrix are zeros
     const auto place = [&](uint32_t c, uint32_t r) { return wide ? (uint64_t)r * S.cols + c0 + c : (uint64_t)(c0 + c) * S.cols + r; };
     const auto each = [&](auto f) {                        // lanes along memory
-        for (uint32_t u = tid; u < NS_SHARE * NS_SIDE; u += NS_THREADS) { const uint32_t c = wide ? u % NS_SHARE : u / NS_SIDE, r = wide ? u / NS_SHARE : u % NS_SIDE; f(c, r, c < mine && r < m); }
+        for (uint32_t u = tid; u < padded * NS_SIDE; u += NS_THREADS) { const uint32_t c = wide ? u % padded : u / NS_SIDE, r = wide ? u / padded : u % NS_SIDE; f(c, r, c < mine && r < m); }
     };
     double sq = 0.0;
     each([&](uint32_t c, uint32_t r, bool in) {
@@ -233,6 +235,7 @@ k_ns_small(const __grid_constant__ NsSmall S) {
         {   // P = X_r X_r^T: 8 x 4 sums a thread
             const uint32_t r0 = warp * 8, q0 = lane * 4;
             float acc[8][4] = {};
+            if (r0 < m)
 #pragma unroll 2
             for (uint32_t k = 0; k < mine; k++) {
                 const float4 a0 = *reinterpret_cast<const float4 *>(&X[k][r0]), a1 = *reinterpret_cast<const float4 *>(&X[k][r0 + 4]), b = *reinterpret_cast<const float4 *>(&X[k][q0]);
@@ -259,33 +262,29 @@ k_ns_small(const __grid_constant__ NsSmall S) {
             __syncthreads();
         }
         hg::cluster_sync();
-        // its rows of a I + b A + c A A: a warp sums an equal share of the contraction for eight whole rows, the parts are added in warp order
+        // its rows of a I + b A + c A A: a warp sums a quarter of the contraction for two whole rows, the parts are added in order
         for (uint32_t i0 = 0; i0 < band; i0 += 8) {
-            const uint32_t r0 = rank * band + i0;
-            float4 acc[8];
+            const uint32_t r0 = rank * band + i0 + (warp & 3u) * 2, k1 = (warp >> 2) * 32;
+            float4 acc[2] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
+            if (r0 < m)
+#pragma unroll 2
+                for (uint32_t k = k1; k < k1 + 32; k += 4) {
+                    const float4 a0 = *reinterpret_cast<const float4 *>(&A[r0][k]), a1 = *reinterpret_cast<const float4 *>(&A[r0 + 1][k]);
+                    const float u[4] = {a0.x, a0.y, a0.z, a0.w}, v[4] = {a1.x, a1.y, a1.z, a1.w};
 #pragma unroll
-            for (int i = 0; i < 8; i++) acc[i] = make_float4(0, 0, 0, 0);
-#pragma unroll
-            for (uint32_t k0 = 0; k0 < NS_SIDE / NS_WARPS; k0 += 4) {
-                const uint32_t k = warp * (NS_SIDE / NS_WARPS) + k0;
-                float4 b[4];
-#pragma unroll
-                for (int j = 0; j < 4; j++) b[j] = *reinterpret_cast<const float4 *>(&A[k + j][lane * 4]);
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float4 a = *reinterpret_cast<const float4 *>(&A[r0 + i][k]);
-                    const float av[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-                    for (int j = 0; j < 4; j++) { acc[i].x += av[j] * b[j].x; acc[i].y += av[j] * b[j].y; acc[i].z += av[j] * b[j].z; acc[i].w += av[j] * b[j].w; }
+                    for (int j = 0; j < 4; j++) {
+                        const float4 b = *reinterpret_cast<const float4 *>(&A[k + j][lane * 4]);
+                        acc[0].x += u[j] * b.x; acc[0].y += u[j] * b.y; acc[0].z += u[j] * b.z; acc[0].w += u[j] * b.w;
+                        acc[1].x += v[j] * b.x; acc[1].y += v[j] * b.y; acc[1].z += v[j] * b.z; acc[1].w += v[j] * b.w;
+                    }
                 }
-            }
 #pragma unroll
-            for (int i = 0; i < 8; i++) parts[(warp * 8 + i) * 32 + lane] = acc[i];
+            for (int i = 0; i < 2; i++) parts[((warp >> 2) * 8 + (warp & 3u) * 2 + i) * 32 + lane] = acc[i];
             __syncthreads();
-            const uint32_t r = r0 + (warp & 7u), c = lane * 4, side = warp >> 3, some = ranks / 2;
+            const uint32_t r = rank * band + i0 + (warp & 7u), c = lane * 4, side = warp >> 3, some = ranks / 2;
             float4 s = make_float4(0, 0, 0, 0);
 #pragma unroll
-            for (uint32_t w = 0; w < NS_WARPS; w++) { const float4 v = parts[(w * 8 + (warp & 7u)) * 32 + lane]; s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w; }
+            for (uint32_t w = 0; w < 4; w++) { const float4 v = parts[(w * 8 + (warp & 7u)) * 32 + lane]; s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w; }
             const float4 q = *reinterpret_cast<const float4 *>(&A[r][c]);
             s.x = NS_B * q.x + NS_C * s.x + (r == c ? NS_A : 0.0f); s.y = NS_B * q.y + NS_C * s.y + (r == c + 1 ? NS_A : 0.0f);
             s.z = NS_B * q.z + NS_C * s.z + (r == c + 2 ? NS_A : 0.0f); s.w = NS_B * q.w + NS_C * s.w + (r == c + 3 ? NS_A : 0.0f);
@@ -294,26 +293,25 @@ k_ns_small(const __grid_constant__ NsSmall S) {
             __syncthreads();
         }
         hg::cluster_sync();
-        {   // X_r = B X_r: 4 rows x 2 columns a thread; B is symmetric to rounding, so its rows are read as columns
-            const uint32_t r0 = lane * 4, q0 = warp * 2;
+        // X_r = B X_r: 4 rows x 2 columns of every 32 a thread; B is symmetric to rounding, so its rows are read as columns.  The columns
+        // are independent of one another and a warp's belong to it alone: they are replaced as they are done
+        for (uint32_t q0 = warp * 2; q0 < mine; q0 += 2 * NS_WARPS) {
+            const uint32_t r0 = lane * 4;
             float acc[2][4] = {};
-            if (q0 < mine) {
 #pragma unroll 2
-                for (uint32_t k = 0; k < m; k += 4) {      // (rows and columns beyond m are zeros)
-                    const float4 x0 = *reinterpret_cast<const float4 *>(&X[q0][k]), x1 = *reinterpret_cast<const float4 *>(&X[q0 + 1][k]);
-                    const float u[4] = {x0.x, x0.y, x0.z, x0.w}, v[4] = {x1.x, x1.y, x1.z, x1.w};
+            for (uint32_t k = 0; k < m; k += 4) {          // (rows and columns beyond m are zeros)
+                const float4 x0 = *reinterpret_cast<const float4 *>(&X[q0][k]), x1 = *reinterpret_cast<const float4 *>(&X[q0 + 1][k]);
+                const float u[4] = {x0.x, x0.y, x0.z, x0.w}, v[4] = {x1.x, x1.y, x1.z, x1.w};
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const float4 b = *reinterpret_cast<const float4 *>(&B[k + j][r0]);
-                        acc[0][0] += b.x * u[j]; acc[0][1] += b.y * u[j]; acc[0][2] += b.z * u[j]; acc[0][3] += b.w * u[j];
-                        acc[1][0] += b.x * v[j]; acc[1][1] += b.y * v[j]; acc[1][2] += b.z * v[j]; acc[1][3] += b.w * v[j];
-                    }
+                for (int j = 0; j < 4; j++) {
+                    const float4 b = *reinterpret_cast<const float4 *>(&B[k + j][r0]);
+                    acc[0][0] += b.x * u[j]; acc[0][1] += b.y * u[j]; acc[0][2] += b.z * u[j]; acc[0][3] += b.w * u[j];
+                    acc[1][0] += b.x * v[j]; acc[1][1] += b.y * v[j]; acc[1][2] += b.z * v[j]; acc[1][3] += b.w * v[j];
                 }
             }
-            __syncthreads();
-            if (q0 < mine)
+            __syncwarp();
 #pragma unroll
-                for (int j = 0; j < 2; j++) *reinterpret_cast<float4 *>(&X[q0 + j][r0]) = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
+            for (int j = 0; j < 2; j++) *reinterpret_cast<float4 *>(&X[q0 + j][r0]) = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
         }
     }
     __syncthreads();
