@@ -22,7 +22,7 @@
 // or m / n along memory rows (boxes of 64 rows x 64 k), so nothing is ever transposed.
 //
 // What bounds it, measured: the tensor cores, and the power they draw.  8192 x 4096 x 4096 in f16 207 us, 1326 TFLOP/s, 0.80 of the measured
-// burst rate (in a loop the clock falls to 1.35 GHz: 250 us); 4096^3 in f32 358 us with the planes' making, 385 TFLOP/s, of which
+// burst rate (in a long loop the clock falls to 1.35 GHz: 250 to 270 us); 4096^3 in f32 358 us with the planes' making, 385 TFLOP/s, of which
 // three f16 MMAs each make 1154.  A pair takes 1900 cycles for 64 k of three products, whose MMAs take 1536: the rest is the epilogue where the
 // next tile's first two chunks do not hide it, and tile loads and MMAs sharing shared memory's bandwidth (without loads 1640).
 //
@@ -203,22 +203,23 @@ __device__ __forceinline__ void put_block(Epi &e, float *st, uint32_t lane, uint
         if (!WHOLE && n >= N) return;
         e.template column<4>(n);
         float *p = st + ro * 32u;
-#pragma unroll
-        for (uint32_t t = 0; t < 8; t += 4) {          // row ro + 4 t: swap(ro + 4 t) = ro ^ (4 (t & 1)) ^ t
+        constexpr int TIMES = Epi::heavy ? 1 : 2;      // (gelu: 121 us as a loop, 127 unrolled; without an activation 103 and 104, f16 43 and 38)
+#pragma unroll TIMES
+        for (uint32_t t = 0; t < 8; t += 4) {          // row ro + 4 (t + i): swap of it = ro ^ (4 (i & 1)) ^ i ^ t
             float x[4][4], v[4][4];
 #pragma unroll
             for (uint32_t i = 0; i < 4; i++)
                 if (m0 + ro + 4 * (t + i) < M) e.template fetch<4>(m0 + ro + 4 * (t + i), n, x[i]);
 #pragma unroll
             for (uint32_t i = 0; i < 4; i++) {
-                const float4 q = *reinterpret_cast<const float4 *>(p + (t + i) * 128u + ((b ^ (((i & 1u) * 4u) ^ (t + i))) << 2));
+                const float4 q = *reinterpret_cast<const float4 *>(p + (t + i) * 128u + ((b ^ t ^ (((i & 1u) * 4u) ^ i)) << 2));
                 v[i][0] = q.x; v[i][1] = q.y; v[i][2] = q.z; v[i][3] = q.w;
             }
             e.template put<4, 4>(Rows{m0 + ro + 4 * t, 4, M}, n, v, x, z);
             if constexpr (Epi::mirrors) {              // the finished values go back, for the mirror to store
 #pragma unroll
                 for (uint32_t i = 0; i < 4; i++)
-                    *reinterpret_cast<float4 *>(p + (t + i) * 128u + ((b ^ (((i & 1u) * 4u) ^ (t + i))) << 2)) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
+                    *reinterpret_cast<float4 *>(p + (t + i) * 128u + ((b ^ t ^ (((i & 1u) * 4u) ^ i)) << 2)) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
             }
         }
     } else {
@@ -439,7 +440,7 @@ k_hgemm(const __grid_constant__ Shape S, const __grid_constant__ Maps maps, cons
 
 // Sums of a split product: partial[z][m][n] in split order, then the epilogue.
 struct PartialEpi {
-    static constexpr bool mirrors = false, long_start = false;
+    static constexpr bool mirrors = false, long_start = false, heavy = false;
     float *partial; uint64_t mn; uint32_t N;
     __device__ bool wide() const { return N % 4 == 0; }
     __device__ float row_factor(uint32_t) const { return 1.0f; }

@@ -5,7 +5,7 @@
 //
 // Three ways, by size: a few rows on the CUDA cores with the weights streamed once (k_linear_few); small products in one launch on the CUDA
 // cores (layer_small.cuh); the rest on the matrix engine (hgemm.cuh), f16 operands as they lie in memory, f32 ones as two f16 planes that
-// kernels of this file make first.  Forward 4096 x 1024 -> 4096, f32, gelu, z kept: 136 us, 17 of them the planes; its backward pass
+// kernels of this file make first.  Forward 4096 x 1024 -> 4096, f32, gelu, z kept: 121 us, 17 of them the planes; its backward pass
 // 255 us: dz and its planes 40, x's 31, w's 8, bias 7, the two products 166.
 #include "hgemm.cuh"
 #include "layer_common.cuh"
@@ -278,7 +278,7 @@ template <typename T, int V, int R> __device__ __forceinline__ void store_rows(T
     for (uint32_t i = 0; i < R; i++, p += step) if (r.first + i * r.step < r.end) store_vec<V>(p, v[i]);
 }
 template <typename T, uint32_t ACT> struct LayerEpi {  // act(sum 2^-exps[m] + bias) + residual
-    static constexpr bool mirrors = false, long_start = false;
+    static constexpr bool mirrors = false, long_start = false, heavy = ACT == THC_ACT_GELU || ACT == THC_ACT_SILU;
     T *out, *z; const T *bias, *residual; const int *exps; uint32_t N;
     float bias_n[4];                                   // of the lane's columns
     __device__ bool wide() const { return N % 4 == 0; }
@@ -303,7 +303,7 @@ template <typename T, uint32_t ACT> struct LayerEpi {  // act(sum 2^-exps[m] + b
     }
 };
 template <typename T, bool COLS> struct GradEpi {      // sum 2^(-exps[m] - col_exps[n])
-    static constexpr bool mirrors = false, long_start = false;
+    static constexpr bool mirrors = false, long_start = false, heavy = false;
     T *out; const int *exps, *col_exps; uint32_t N;
     int exp_n[4];
     __device__ bool wide() const { return N % 4 == 0; }

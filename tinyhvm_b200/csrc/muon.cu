@@ -4,8 +4,8 @@
 // with the quintic's coefficients a, b, c = 3.4445, -4.7750, 2.0315: X keeps G's singular vectors and its singular values
 // move to the neighbourhood of 1.
 // On the matrix engine a step is three products, with the matrices between them kept as the engine's f16 planes: A and B are symmetric and
-// only made from the diagonal on.  Five steps: 4096 x 4096 3.7 ms (1374 GFLOP with
-// the symmetry used: 375 TFLOP/s, 1125 of f16 products, the clock at its power limit); 1024 x 4096 370 us.
+// only made from the diagonal on.  Five steps: 4096 x 4096 3.9 ms (1374 GFLOP with
+// the symmetry used: 353 TFLOP/s, 1060 of f16 products, the clock at its power limit); 1024 x 4096 390 us.
 //   mom = mu mom + g;  u = nesterov ? g + mu mom : mom;  p = p (1 - lr decay) - lr sqrt(max(1, rows / cols)) X(u)
 #include <math.h>
 #include "hgemm.cuh"
@@ -98,7 +98,7 @@ template <int V, int R> __device__ __forceinline__ void put_planes(__half *hi, _
     for (uint32_t i = 0; i < R; i++) if (r.first + i * r.step < r.end) store_planes<V>(hi + at + i * step, lo + at + i * step, v[i]);
 }
 struct SquareEpi {                                     // A = X X^T
-    static constexpr bool mirrors = true, long_start = false;
+    static constexpr bool mirrors = true, long_start = false, heavy = false;
     __half *hi, *lo; uint64_t pitch; uint32_t side;
     __device__ bool wide() const { return side % 4 == 0; }
     __device__ float row_factor(uint32_t) const { return 1.0f / PLANE; }
@@ -109,7 +109,7 @@ struct SquareEpi {                                     // A = X X^T
     template <int V, int R> __device__ void mirror(hg::Rows r, uint32_t m, const float (&v)[R][V]) const { put_planes<V, R>(hi, lo, pitch, r, m, v); }
 };
 struct PolyEpi {                                       // b A + c A A
-    static constexpr bool mirrors = true, long_start = false;
+    static constexpr bool mirrors = true, long_start = false, heavy = false;
     __half *hi, *lo; const __half *a_hi, *a_lo; uint64_t pitch; uint32_t side;
     __device__ bool wide() const { return side % 4 == 0; }
     __device__ float row_factor(uint32_t) const { return 1.0f / PLANE; }
@@ -135,7 +135,7 @@ enum { NEXT, RESULT, STEP };
 // X = a X + (b A + c A A) X: planes for the next step, the result, or the parameters' step.  a X is added here, in f32: it is most of the sum
 // while the small singular values still grow, and the tensor core's truncation would be a share of it.
 template <int TO> struct ApplyEpi {
-    static constexpr bool mirrors = false, long_start = true;
+    static constexpr bool mirrors = false, long_start = true, heavy = false;
     const __half *x_hi, *x_lo; __half *hi, *lo; uint64_t pitch;
     float *out; uint32_t cols; float keep, step;
     __device__ bool wide() const { return cols % 4 == 0; }
