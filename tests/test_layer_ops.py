@@ -335,6 +335,26 @@ def test_linear_keeps_f32_over_wide_ranges(host, M):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N", [(40, 64, 48), (520, 640, 704)])
+def test_linear_beside_rows_of_zeros(host, M, K, N):
+    """Rows of w, of x or of dy that are zero (pruned inputs, masked tokens) cost the other rows no precision, however small those are."""
+    rng = np.random.default_rng(11)
+    x, w, dy = rng.standard_normal((M, K)), 1e-6 * rng.standard_normal((K, N)), 1e-9 * rng.standard_normal((M, N))
+    x[::5], w[::2], dy[::3] = 0.0, 0.0, 0.0
+    x, w, dy = (a.astype(np.float32) for a in (x, w, dy))
+    bx, bw, bdy = host.up(x), host.up(w), host.up(dy)
+    by, bdx, bdw, bdb = (host.out(n) for n in (M * N, M * K, K * N, N))
+    assert host.lib.thvm_cuda_linear(by, 0, bx, bw, 0, 0, M, K, N, NONE, F32) == 0
+    assert host.lib.thvm_cuda_linear_backward(bdx, bdw, bdb, bdy, 0, bx, bw, M, K, N, NONE, F32) == 0
+    x, w, dy = (a.astype(np.float64) for a in (x, w, dy))
+    for bid, want, S, n in ((by, x @ w, np.abs(x) @ np.abs(w), K), (bdx, dy @ w.T, np.abs(dy) @ np.abs(w).T, N), (bdw, x.T @ dy, np.abs(x).T @ np.abs(dy), M), (bdb, dy.sum(0), np.abs(dy).sum(0), M)):
+        got = host.get(bid, want.shape)
+        near(got, want, product_slack(n, S))
+        assert norm2(got, want) <= 2e-6
+    host.done()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("M", [2, 300])
 def test_linear_zero_and_nan_rows(host, M):
     """A row of zeros gives act(bias); a NaN stays in its own row of y."""

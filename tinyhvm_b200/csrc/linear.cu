@@ -53,11 +53,12 @@ bool layer_buffers(const char *who, const uint32_t *ins, const uint64_t *in_need
 //   dw        dz [M,N] by rows m: dz' = dz 2^s_m;        x' = x 2^-s_m, then scaled by its columns k (over m)
 // Values below 2^-40 of the largest in their row (column) are rounded to that step.  An infinity in an f32 operand of the
 // matrix engine gives NaN where it takes part, as in the framework's other contractions: its low part is no number.
-__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }       // -126 <= e <= 127
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }       // -126 <= e <= 127; 0 at -127
 __device__ __forceinline__ float finite_abs(float v) { v = fabsf(v); return v <= 3.402823466e38f ? v : 0.0f; }
-// the exponent s that puts `top` into [2^14, 2^15); rows below 2^-112 keep fewer bits
+// the exponent s that puts `top` into [2^14, 2^15); rows below 2^-112 keep fewer bits.  A row of zeros gets 127, whose way back is a factor
+// of 0: what the other operand has beside it (a masked token's values) has no part in that operand's own scale.
 __device__ __forceinline__ int scale_for(float top) {
-    if (top == 0.0f) return 0;
+    if (top == 0.0f) return 127;
     const int s = 14 - ((int)(__float_as_uint(top) >> 23) - 127);
     return s > 126 ? 126 : s;
 }
